@@ -41,6 +41,37 @@ namespace {
 inline hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// Bytes [first, last) that rows of `width` bytes take at a stride.
+struct ByteRows {
+  uintptr_t first = 0, last = 0;
+  uint64_t stride = 0, width = 0;
+};
+ByteRows byte_rows(const void* data, int64_t rows, int64_t stride, int64_t cols, int64_t size) {
+  ByteRows r;
+  if (data == nullptr || rows <= 0 || cols <= 0) return r;
+  r.first = reinterpret_cast<uintptr_t>(data);
+  r.stride = (uint64_t)(stride * size);
+  r.width = (uint64_t)(cols * size);
+  r.last = r.first + (uint64_t)(rows - 1) * r.stride + r.width;
+  return r;
+}
+// Whether two sets of rows share a byte.  Sets whose ranges cross do not where
+// they are columns apart of the rows of one buffer (equal strides).
+bool overlap(const ByteRows& a, const ByteRows& b) {
+  if (a.first >= b.last || b.first >= a.last) return false;
+  if (a.stride != b.stride || a.width > a.stride || b.width > b.stride) return true;
+  const uint64_t d = a.first <= b.first ? (b.first - a.first) % a.stride
+                                        : (a.stride - (a.first - b.first) % a.stride) % a.stride;
+  return d < a.width || a.stride - d < b.width;
+}
+
+constexpr int64_t kMaxDim = 0x7fffffff;
+// Row strides are held to 2^40 elements, so that no byte range overflows.
+constexpr int64_t kMaxStride = (int64_t)1 << 40;
+bool stride_ok(int64_t stride, int64_t cols, int64_t rows) {
+  return rows <= 1 || (stride >= cols && stride <= kMaxStride / rows);
+}
+
 }  // namespace
 }  // namespace gd
 
@@ -252,6 +283,197 @@ int gd_deberta_attention(gd_bhld q, gd_bhld k, gd_bhld v, gd_table pos_key, gd_t
   const float scale_rel = head_dim > 0 ? 1.0f / std::sqrt((float)(3 * head_dim)) : 0.f;
   return deberta_attention_checked(q, k, v, pos_key, pos_query, mask, mask_kind, batch, heads, seq_len, head_dim,
                                    positions, bucket_size, kind, score, scale_rel, out, ldo, as_stream(stream));
+}
+
+int64_t gd_packed_attention_workspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int64_t heads,
+                                      int64_t kv_heads, int64_t head_dim) {
+  if (batch <= 0 || q_tokens <= 0 || k_tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  if (batch > kMaxDim || q_tokens > kMaxDim || k_tokens > kMaxDim || heads > 4096 || heads % kv_heads != 0 ||
+      head_dim > 256)
+    return 0;
+  return packed_attention_workspace(batch, q_tokens, k_tokens, heads, kv_heads, head_dim);
+}
+
+int gd_packed_attention(gd_tokens q, gd_tokens k, gd_tokens v, const int32_t* q_offsets, const int32_t* k_offsets,
+                        int64_t batch, int64_t q_tokens, int64_t k_tokens, int64_t heads, int64_t kv_heads,
+                        int64_t head_dim, int32_t dtype, float scale, uint32_t flags, void* out, int64_t ldo,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  GD_CHECK_ARG(dtype == GD_F16 || dtype == GD_BF16, "dtype must be GD_F16 or GD_BF16 (got %d)", dtype);
+  GD_CHECK_ARG((flags & ~(GD_PACKED_CAUSAL | GD_PACKED_ZERO_REST)) == 0, "unknown flags 0x%x", flags);
+  GD_CHECK_ARG(std::isfinite(scale), "scale must be finite");
+  GD_CHECK_SHAPE(batch >= 0 && q_tokens >= 0 && k_tokens >= 0 && batch < kMaxDim && q_tokens <= kMaxDim &&
+                     k_tokens <= kMaxDim,
+                 "batch and token counts must be in [0, 2^31)");
+  GD_CHECK_SHAPE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 4096,
+                 "heads must be a positive multiple of kv_heads, at most 4096 (got %lld, %lld)", (long long)heads,
+                 (long long)kv_heads);
+  GD_CHECK_SHAPE(head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 192 ||
+                     head_dim == 256,
+                 "head_dim must be 32, 64, 96, 128, 192 or 256 (got %lld)", (long long)head_dim);
+  GD_CHECK_SHAPE(k_offsets || k_tokens == q_tokens, "without k_offsets the keys are the queries' own tokens");
+  GD_CHECK_SHAPE(ldo >= heads * head_dim && ldo % 8 == 0 && ldo <= kMaxStride / (q_tokens + 1),
+                 "ldo must be a multiple of 8 and at least heads * head_dim");
+  const gd_tokens* views[3] = {&q, &k, &v};
+  for (int i = 0; i < 3; ++i) {
+    const gd_tokens* t = views[i];
+    const int64_t tokens = i == 0 ? q_tokens : k_tokens, nh = i == 0 ? heads : kv_heads;
+    GD_CHECK_ARG(aligned(t->data, 16) && t->stride_t % 8 == 0 && t->stride_h % 8 == 0,
+                 "q/k/v must be 16-byte aligned with strides that are multiples of 8 elements");
+    GD_CHECK_SHAPE(t->stride_t >= 0 && t->stride_h >= 0 && t->stride_t <= kMaxStride / (tokens + 1) &&
+                       t->stride_h <= kMaxStride / nh,
+                   "q/k/v strides must not be negative");
+  }
+  if (q_tokens == 0) return GD_OK;
+  GD_CHECK_ARG(q.data && q_offsets && out, "null tensor pointer");
+  GD_CHECK_ARG(k_tokens == 0 || (k.data && v.data), "null tensor pointer");
+  GD_CHECK_ARG(aligned(out, 16) && aligned(workspace, 16), "out and workspace must be 16-byte aligned");
+  GD_CHECK_ARG(aligned(q_offsets, 4) && aligned(k_offsets, 4), "offsets must be aligned int32");
+  const ByteRows o = byte_rows(out, q_tokens, ldo, heads * head_dim, 2);
+  for (int i = 0; i < 3; ++i) {
+    const gd_tokens* t = views[i];
+    const int64_t tokens = i == 0 ? q_tokens : k_tokens, nh = i == 0 ? heads : kv_heads;
+    GD_CHECK_ARG(!overlap(o, byte_rows(t->data, tokens, t->stride_t, (nh - 1) * t->stride_h + head_dim, 2)),
+                 "out must not overlap q, k or v");
+  }
+  PackedAttentionArgs a{};
+  a.q = q.data;
+  a.k = k.data;
+  a.v = v.data;
+  a.qst = q.stride_t;
+  a.qsh = q.stride_h;
+  a.kst = k.stride_t;
+  a.ksh = k.stride_h;
+  a.vst = v.stride_t;
+  a.vsh = v.stride_h;
+  a.q_off = q_offsets;
+  a.k_off = k_offsets ? k_offsets : q_offsets;
+  a.B = batch;
+  a.Tq = q_tokens;
+  a.Tk = k_tokens;
+  a.Hq = heads;
+  a.Hk = kv_heads;
+  a.D = head_dim;
+  a.scale = scale;
+  a.causal = (flags & GD_PACKED_CAUSAL) != 0;
+  a.zero_rest = (flags & GD_PACKED_ZERO_REST) != 0;
+  a.bf16 = dtype == GD_BF16;
+  a.out = out;
+  a.ldo = ldo;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace ? workspace_bytes : 0;
+  return launch_packed_attention(a, as_stream(stream));
+}
+
+int gd_projection(gd_rows x, gd_rows w, const void* bias, gd_rows residual, void* out, int64_t ldo, int64_t m,
+                  int64_t n, int64_t k, int32_t activation, float scale, int32_t dtype, void* stream) {
+  clear_error();
+  GD_CHECK_ARG(dtype == GD_F16 || dtype == GD_BF16, "dtype must be GD_F16 or GD_BF16 (got %d)", dtype);
+  GD_CHECK_ARG(activation >= GD_ACT_NONE && activation <= GD_ACT_SILU, "unknown activation %d", activation);
+  GD_CHECK_ARG(std::isfinite(scale), "scale must be finite");
+  GD_CHECK_SHAPE(m >= 0 && n >= 0 && k > 0 && m <= kMaxDim && n <= kMaxDim && k <= kMaxDim,
+                 "m, n must be in [0, 2^31) and k in [1, 2^31) (got %lld, %lld, %lld)", (long long)m, (long long)n,
+                 (long long)k);
+  GD_CHECK_SHAPE(stride_ok(x.stride, k, m) && stride_ok(w.stride, k, n) && stride_ok(ldo, n, m) &&
+                     (!residual.data || stride_ok(residual.stride, n, m)),
+                 "row strides must be at least the rows' lengths");
+  if (m == 0 || n == 0) return GD_OK;
+  GD_CHECK_ARG(x.data && w.data && out, "null tensor pointer");
+  GD_CHECK_ARG(aligned(x.data, 2) && aligned(w.data, 2) && aligned(bias, 2) && aligned(residual.data, 2) &&
+                   aligned(out, 2),
+               "tensors must be aligned to their elements");
+  const ByteRows o = byte_rows(out, m, ldo, n, 2);
+  GD_CHECK_ARG(!overlap(o, byte_rows(x.data, m, x.stride, k, 2)) &&
+                   !overlap(o, byte_rows(w.data, n, w.stride, k, 2)) && !overlap(o, byte_rows(bias, 1, n, n, 2)),
+               "out must not overlap x, w or bias");
+  GD_CHECK_ARG((out == residual.data && (ldo == residual.stride || m == 1)) ||
+                   !overlap(o, byte_rows(residual.data, m, residual.stride, n, 2)),
+               "out must be the residual itself or not overlap it");
+  ProjectionArgs a{};
+  a.x = x.data;
+  a.w = w.data;
+  a.bias = bias;
+  a.residual = residual.data;
+  a.ldx = x.stride;
+  a.ldw = w.stride;
+  a.ldr = residual.stride;
+  a.out = out;
+  a.ldo = ldo;
+  a.m = m;
+  a.n = n;
+  a.k = k;
+  a.activation = activation;
+  a.scale = scale;
+  a.bf16 = dtype == GD_BF16;
+  return launch_projection(a, as_stream(stream));
+}
+
+int gd_block_norm(gd_rows y, gd_rows residual, gd_rows gate, int64_t rows_per_gate, const void* post_weight,
+                  const void* post_bias, const void* pre_weight, const void* pre_bias, void* h, int64_t ldh, void* n,
+                  int64_t ldn, int64_t rows, int64_t cols, float eps, float scale, int32_t kind, int32_t dtype,
+                  int32_t stream_dtype, void* stream) {
+  clear_error();
+  GD_CHECK_ARG(dtype == GD_F16 || dtype == GD_BF16, "dtype must be GD_F16 or GD_BF16 (got %d)", dtype);
+  GD_CHECK_ARG(stream_dtype == dtype || stream_dtype == GD_F32, "stream_dtype must be dtype or GD_F32 (got %d)",
+               stream_dtype);
+  GD_CHECK_ARG(kind == GD_NORM_LAYER || kind == GD_NORM_RMS, "unknown norm %d", kind);
+  GD_CHECK_ARG(eps > 0.f && std::isfinite(eps), "eps must be positive and finite");
+  GD_CHECK_ARG(std::isfinite(scale), "scale must be finite");
+  GD_CHECK_ARG(post_weight || !post_bias, "post_bias needs post_weight");
+  GD_CHECK_SHAPE(rows >= 0 && rows <= kMaxDim, "rows must be in [0, 2^31) (got %lld)", (long long)rows);
+  GD_CHECK_SHAPE(cols >= 1 && cols <= 32768, "cols must be in [1, 32768] (got %lld)", (long long)cols);
+  GD_CHECK_SHAPE(!gate.data || rows_per_gate > 0, "rows_per_gate must be positive");
+  const int64_t gates = gate.data && rows > 0 ? (rows - 1) / rows_per_gate + 1 : 0;
+  GD_CHECK_SHAPE(stride_ok(y.stride, cols, rows) && stride_ok(residual.stride, cols, rows) &&
+                     stride_ok(ldh, cols, rows) && stride_ok(ldn, cols, rows) && stride_ok(gate.stride, cols, gates),
+                 "row strides must be at least cols");
+  if (rows == 0) return GD_OK;
+  GD_CHECK_ARG(y.data && residual.data && pre_weight && h && n, "null tensor pointer");
+  const int64_t ss = stream_dtype == GD_F32 ? 4 : 2;
+  GD_CHECK_ARG(aligned(y.data, 2) && aligned(gate.data, 2) && aligned(post_weight, 2) && aligned(post_bias, 2) &&
+                   aligned(pre_weight, 2) && aligned(pre_bias, 2) && aligned(n, 2) && aligned(h, ss) &&
+                   aligned(residual.data, ss),
+               "tensors must be aligned to their elements");
+  const ByteRows rh = byte_rows(h, rows, ldh, cols, ss), rn = byte_rows(n, rows, ldn, cols, 2);
+  GD_CHECK_ARG(!overlap(rh, rn), "h and n must not overlap");
+  const ByteRows rest[5] = {byte_rows(gate.data, gates, gate.stride, cols, 2), byte_rows(post_weight, 1, cols, cols, 2),
+                             byte_rows(post_bias, 1, cols, cols, 2), byte_rows(pre_weight, 1, cols, cols, 2),
+                             byte_rows(pre_bias, 1, cols, cols, 2)};
+  for (const ByteRows& r : rest)
+    GD_CHECK_ARG(!overlap(rh, r) && !overlap(rn, r), "h and n must not overlap the gate, weights or biases");
+  const gd_rows in[2] = {y, residual};
+  for (int i = 0; i < 2; ++i) {
+    const int64_t size = i == 0 ? 2 : ss;
+    const ByteRows r = byte_rows(in[i].data, rows, in[i].stride, cols, size);
+    const bool same_h = h == in[i].data && size == ss && (ldh == in[i].stride || rows == 1);
+    const bool same_n = n == in[i].data && size == 2 && (ldn == in[i].stride || rows == 1);
+    GD_CHECK_ARG((same_h || !overlap(rh, r)) && (same_n || !overlap(rn, r)),
+                 "h and n must be y or the residual themselves or not overlap them");
+  }
+  BlockNormArgs a{};
+  a.y = y.data;
+  a.residual = residual.data;
+  a.gate = gate.data;
+  a.post_w = post_weight;
+  a.post_b = post_bias;
+  a.pre_w = pre_weight;
+  a.pre_b = pre_bias;
+  a.h = h;
+  a.n = n;
+  a.ldy = y.stride;
+  a.ldr = residual.stride;
+  a.ldg = gate.stride;
+  a.ldh = ldh;
+  a.ldn = ldn;
+  a.rows_per_gate = gate.data ? rows_per_gate : 1;
+  a.rows = rows;
+  a.cols = cols;
+  a.eps = eps;
+  a.scale = scale;
+  a.rms = kind == GD_NORM_RMS;
+  a.bf16 = dtype == GD_BF16;
+  a.stream_f32 = stream_dtype == GD_F32;
+  return launch_block_norm(a, as_stream(stream));
 }
 
 int gd_stream_probe_add(const void* a, const void* b, void* c, int64_t n, void* stream) {

@@ -136,6 +136,44 @@ int launch_fused_attention_general(const void* q, const void* k, const void* v, 
                                    float scale, int64_t B, int64_t H, int64_t L, int64_t D, int64_t P, void* out,
                                    int32_t* error_flag, hipStream_t stream);
 
+// Attention over packed sequences (packed_attention.hip); strides in elements.
+struct PackedAttentionArgs {
+  const void *q, *k, *v;
+  int64_t qst, qsh, kst, ksh, vst, vsh;
+  const int32_t *q_off, *k_off;  // [B + 1]
+  int64_t B, Tq, Tk, Hq, Hk, D;
+  float scale;
+  bool causal, zero_rest, bf16;
+  void* out;
+  int64_t ldo;
+  void* workspace;
+  int64_t workspace_bytes;
+};
+int64_t packed_attention_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D);
+int launch_packed_attention(const PackedAttentionArgs& args, hipStream_t stream);
+
+// out = residual + scale * act(x w^T + bias) (projection.hip); strides in elements.
+struct ProjectionArgs {
+  const void *x, *w, *bias, *residual;
+  int64_t ldx, ldw, ldr, ldo;
+  void* out;
+  int64_t m, n, k;
+  int activation;
+  float scale;
+  bool bf16;
+};
+int launch_projection(const ProjectionArgs& args, hipStream_t stream);
+
+// h = residual + scale * gate * post(y), n = pre(h) (block_norm.hip); strides in elements.
+struct BlockNormArgs {
+  const void *y, *residual, *gate, *post_w, *post_b, *pre_w, *pre_b;
+  void *h, *n;
+  int64_t ldy, ldr, ldg, ldh, ldn, rows_per_gate, rows, cols;
+  float eps, scale;
+  bool rms, bf16, stream_f32;
+};
+int launch_block_norm(const BlockNormArgs& args, hipStream_t stream);
+
 int launch_relative_index_table(int32_t* out, int n, int bucket_size, int max_position, hipStream_t stream);
 
 // Classifier head helpers (head.hip).

@@ -46,6 +46,9 @@ GD_F16, GD_F32, GD_BF16, GD_I32, GD_I64 = 0, 1, 2, 3, 4
 GD_LN_SUM_F16 = 1
 GD_EPI_NONE, GD_EPI_BIAS, GD_EPI_BIAS_GELU, GD_EPI_BIAS_RELU = 0, 1, 2, 3
 GD_MASK_ATTENTION, GD_MASK_ADDITIVE = 0, 1
+GD_PACKED_CAUSAL, GD_PACKED_ZERO_REST = 1, 2
+GD_ACT_NONE, GD_ACT_RELU, GD_ACT_GELU, GD_ACT_GELU_TANH, GD_ACT_SILU = 0, 1, 2, 3, 4
+GD_NORM_LAYER, GD_NORM_RMS = 0, 1
 GD_ATTN_OUT_PROBS, GD_ATTN_OUT_CONTEXT, GD_ATTN_OUT_BIAS = 0, 1, 2
 GD_ATTN_SCORE_DEFAULT, GD_ATTN_SCORE_EXPLICIT, GD_ATTN_SCORE_KERNEL_BIAS = 0x000, 0x100, 0x200
 GD_ATTN_SCORE_KERNEL_BIAS_EXPLICIT, GD_ATTN_SCORE_FUSED = 0x300, 0x400
@@ -84,6 +87,14 @@ class GdTable(C.Structure):
     _fields_ = [("data", C.c_void_p), ("stride_h", C.c_int64), ("stride_p", C.c_int64)]
 
 
+class GdTokens(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_t", C.c_int64), ("stride_h", C.c_int64)]
+
+
+class GdRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64)]
+
+
 class GdProfileEvent(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("milliseconds", C.c_double)]
 
@@ -107,6 +118,12 @@ _SIGNATURES = {
     "gd_fused_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, f32, i64, i64, i64, i64, i64, vp, vp]),
     "gd_deberta_attention": (C.c_int, [GdBhld, GdBhld, GdBhld, GdTable, GdTable, vp, i32, i64, i64, i64, i64, i64,
                                        i32, i32, vp, i64, vp]),
+    "gd_packed_attention_workspace": (i64, [i64] * 6),
+    "gd_packed_attention": (C.c_int, [GdTokens, GdTokens, GdTokens, vp, vp, i64, i64, i64, i64, i64, i64, i32, f32, u32,
+                                      vp, i64, vp, i64, vp]),
+    "gd_projection": (C.c_int, [GdRows, GdRows, vp, GdRows, vp, i64, i64, i64, i64, i32, f32, i32, vp]),
+    "gd_block_norm": (C.c_int, [GdRows, GdRows, GdRows, i64, vp, vp, vp, vp, vp, i64, vp, i64, i64, i64, f32, f32, i32,
+                                i32, i32, vp]),
     "gd_relative_index_table": (C.c_int, [vp, i32, i32, i32, vp]),
     "gd_stream_probe_add": (C.c_int, [vp, vp, vp, i64, vp]),
     "gd_diag_mfma_forms": (C.c_int, [vp, vp, vp, vp, vp, i64, vp]),

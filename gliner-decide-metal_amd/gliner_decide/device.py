@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import torch
 
+from . import _native as N
+
 
 def require_gpu() -> torch.device:
     if not torch.cuda.is_available():
@@ -56,3 +58,36 @@ def as_i32(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dtype != torch.int32:
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
+
+
+_DTYPES_16 = {torch.float16: N.GD_F16, torch.bfloat16: N.GD_BF16}
+
+
+def dtype16(t: torch.Tensor, name: str) -> int:
+    """gd_dtype of an fp16 or bf16 GPU tensor."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    code = _DTYPES_16.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float16 or bfloat16 (got {t.dtype})")
+    return code
+
+
+def same_kind(t: torch.Tensor, like: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> None:
+    """Refuses a tensor on another device than `like`, or of another type than
+    `dtype` (None: that of `like`)."""
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device} (got {t.device})")
+    dtype = dtype or like.dtype
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+
+
+def call_on(t: torch.Tensor, fn, *args) -> None:
+    """fn(*args, current stream) on t's device, whichever device is current."""
+    index = t.device.index
+    if index == _current_device():
+        N.check(fn(*args, stream_handle()))
+    else:
+        with torch.cuda.device(index):
+            N.check(fn(*args, stream_handle()))

@@ -15,7 +15,7 @@ import math
 import torch
 
 from . import _native as N
-from .device import as_f16, as_i32, ptr, stream_handle
+from .device import as_f16, as_i32, call_on, dtype16, ptr, same_kind, stream_handle
 
 
 def _dims(t: torch.Tensor, n: int, name: str):
@@ -50,6 +50,54 @@ _SCORES = {"default": N.GD_ATTN_SCORE_DEFAULT, "explicit": N.GD_ATTN_SCORE_EXPLI
            "fused": N.GD_ATTN_SCORE_FUSED}
 _MASKS = {"attention": N.GD_MASK_ATTENTION, "additive": N.GD_MASK_ADDITIVE}
 _EPILOGUES = {"none": N.GD_EPI_NONE, "bias": N.GD_EPI_BIAS, "gelu": N.GD_EPI_BIAS_GELU, "relu": N.GD_EPI_BIAS_RELU}
+_ACTIVATIONS = {"none": N.GD_ACT_NONE, "relu": N.GD_ACT_RELU, "gelu": N.GD_ACT_GELU,
+                "gelu_tanh": N.GD_ACT_GELU_TANH, "silu": N.GD_ACT_SILU}
+_NORMS = {"layer": N.GD_NORM_LAYER, "rms": N.GD_NORM_RMS}
+
+
+def _choice(table: dict, key, name: str) -> int:
+    if key not in table:
+        raise N.GlinerDecideError(N.GD_ERR_INVALID_ARGUMENT, f"{name} must be one of {', '.join(table)} (got {key!r})")
+    return table[key]
+
+
+def _tokens(t: torch.Tensor, name: str) -> N.GdTokens:
+    """[T, H, D] with contiguous D; a stride that no element uses is 0."""
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be a [tokens, heads, head_dim] view with contiguous "
+                                                  f"head_dim (got {tuple(t.shape)}, strides {t.stride()})")
+    T, H, _ = t.shape
+    st, sh, _ = t.stride()
+    return N.GdTokens(t.data_ptr(), st if T > 1 else 0, sh if H > 1 else 0)
+
+
+def _rows2(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """[rows, cols] of any leading axes with contiguous, non-overlapping rows (copied where t has none)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.reshape(math.prod(t.shape[:-1]), 0)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def _vector(t: torch.Tensor | None, like: torch.Tensor, n: int, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    same_kind(t, like, name)
+    if t.dim() != 1 or t.shape[0] != n:
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be [{n}] (got {tuple(t.shape)})")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _output(out: torch.Tensor, like: torch.Tensor, shape: tuple, name: str) -> None:
+    """Refuses a given output whose rows (last axis) are not contiguous at one row stride."""
+    same_kind(out, like, name)
+    if tuple(out.shape) != shape:
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be {shape} (got {tuple(out.shape)})")
+    if out.numel() and out.dim() != 2 and not out.is_contiguous():
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be contiguous, or rows with contiguous columns")
+    if out.dim() == 2 and out.shape[1] > 1 and out.stride(1) != 1:
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must have contiguous columns")
 
 
 class FusedKernels:
@@ -206,6 +254,162 @@ class FusedKernels:
         N.check(self._lib.gd_linear(ptr(x2), ptr(w), ptr(b), ptr(out), M, N_, K, K, N_, ptr(rows), x2.shape[0], epi,
                                     stream_handle()))
         return out
+
+    # -- a block over packed rows (no counterpart in the reference) ---------
+    def packed_attention(self, q, k, v, q_offsets, k_offsets=None, *, scale: float | None = None, causal: bool = True,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+        """Softmax attention over packed sequences with grouped heads, fp16 or bf16.
+
+        q: [Tq, H, D], k and v: [Tk, Hk, D] views with contiguous D (the parts
+        of one projection's output, say), H a multiple of Hk, D one of 32, 64,
+        96, 128, 192, 256; head h reads key head h // (H // Hk).  Sequence b
+        holds queries q_offsets[b]:q_offsets[b+1] and keys
+        k_offsets[b]:k_offsets[b+1] (integer GPU tensors [B + 1] that do not
+        decrease; None: the keys are the queries' own tokens).  causal: query i
+        of nq sees the keys j <= nk - nq + i, the last one all of them; a
+        query that sees none gets 0.  scale: of q . k, 1 / sqrt(D) by default.
+
+        Returns [Tq, H, D]; rows of no sequence are 0, in a given `out` (heads
+        contiguous, overlapping no input) they are left as they were.  Forward
+        only: the result carries no gradient."""
+        dtype = dtype16(q, "q")
+        qt, kt, vt = _tokens(q, "q"), _tokens(k, "k"), _tokens(v, "v")
+        same_kind(k, q, "k")
+        same_kind(v, q, "v")
+        Tq, H, D = q.shape
+        Tk, Hk, _ = k.shape
+        if k.shape != v.shape or k.shape[2] != D:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"k and v must both be [tokens, kv_heads, {D}]")
+        q_offsets, batch = self._offsets(q_offsets, q, "q_offsets")
+        if k_offsets is not None:
+            k_offsets, kb = self._offsets(k_offsets, q, "k_offsets")
+            if kb != batch:
+                raise N.GlinerDecideError(N.GD_ERR_SHAPE, "q_offsets and k_offsets must have one length")
+        flags = N.GD_PACKED_CAUSAL if causal else 0
+        if out is None:
+            out = torch.empty((Tq, H, D), dtype=q.dtype, device=q.device)
+            ldo = H * D
+            flags |= N.GD_PACKED_ZERO_REST
+        else:
+            same_kind(out, q, "out")
+            if out.shape != q.shape or (out.numel() and (out.stride(2) != 1 or (H > 1 and out.stride(1) != D))):
+                raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"out must be {tuple(q.shape)} with contiguous heads")
+            ldo = out.stride(0) if Tq > 1 else H * D
+        need = self._lib.gd_packed_attention_workspace(batch, Tq, Tk, H, Hk, D)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        call_on(q, self._lib.gd_packed_attention, qt, kt, vt, q_offsets.data_ptr(),
+                None if k_offsets is None else k_offsets.data_ptr(), batch, Tq, Tk, H, Hk, D, dtype,
+                D ** -0.5 if scale is None else float(scale), flags, out.data_ptr(), ldo,
+                None if work is None else work.data_ptr(), need)
+        return out
+
+    @staticmethod
+    def _offsets(t: torch.Tensor, like: torch.Tensor, name: str):
+        if t.device != like.device:
+            raise ValueError(f"{name} must be on {like.device} (got {t.device})")
+        t = as_i32(t, name)
+        if t.dim() != 1 or t.shape[0] < 1:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be [batch + 1] (got {tuple(t.shape)})")
+        return t, t.shape[0] - 1
+
+    def projection(self, x, weight, bias=None, residual=None, *, activation: str = "none", scale: float = 1.0,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+        """residual + scale * act(x W^T + bias), fp16 or bf16, rounded once.
+
+        x: [..., K], weight: [N, K] (rows at any stride), bias: [N], residual:
+        [..., N]; activation in {"none", "relu", "gelu", "gelu_tanh", "silu"}.
+        Any sizes; rows of 16-byte alignment run faster.  `out` may be the
+        residual itself and overlaps nothing else.  Forward only."""
+        dtype = dtype16(x, "x")
+        same_kind(weight, x, "weight")
+        n, K = _dims(weight, 2, "weight")
+        if x.dim() < 1 or x.shape[-1] != K:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"x {tuple(x.shape)} does not end in the weight's {K} columns")
+        act = _choice(_ACTIVATIONS, activation, "activation")
+        shape = tuple(x.shape[:-1]) + (n,)
+        x2, w = _rows2(x, K), _rows2(weight, K)
+        m = x2.shape[0]
+        bias = _vector(bias, x, n, "bias")
+        res = N.GdRows(None, 0)
+        if residual is not None:
+            same_kind(residual, x, "residual")
+            if tuple(residual.shape) != shape:
+                raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"residual must be {shape} (got {tuple(residual.shape)})")
+            r2 = _rows2(residual, n)
+            res = N.GdRows(r2.data_ptr(), r2.stride(0) if m > 1 else n)
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+            ldo = n
+        else:
+            _output(out, x, shape, "out")
+            ldo = out.stride(0) if out.dim() == 2 and m > 1 else n
+        call_on(x, self._lib.gd_projection, N.GdRows(x2.data_ptr(), x2.stride(0) if m > 1 else K),
+                N.GdRows(w.data_ptr(), w.stride(0) if n > 1 else K), None if bias is None else bias.data_ptr(), res,
+                out.data_ptr(), ldo, m, n, K, act, float(scale), dtype)
+        return out
+
+    def block_norm(self, y, residual, *, pre_weight, pre_bias=None, post_weight=None, post_bias=None, gate=None,
+                   scale: float = 1.0, eps: float = 1e-6, kind: str = "rms", out=None):
+        """(h, n) with h = residual + scale * gate * post(y) and n = pre(h): the
+        norm after a block, its gate and residual scale and the norm before the
+        next block in one pass.
+
+        y: [..., C] fp16 or bf16; residual: its shape, its type or fp32 (h has
+        the residual's type, n has y's); kind "rms" or "layer" for both norms;
+        post_weight=None leaves the first norm out; gate: any shape that
+        broadcasts to y's and keeps C ([C], [B, 1, C] for [B, L, C], y's own).
+        out = (h, n) may be the residual and y themselves.  Forward only."""
+        dtype = dtype16(y, "y")
+        same_kind(residual, y, "residual", torch.float32 if residual.dtype == torch.float32 else None)
+        if y.dim() < 1 or y.shape != residual.shape:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"y {tuple(y.shape)} and residual {tuple(residual.shape)} differ")
+        C = y.shape[-1]
+        shape = tuple(y.shape)
+        code = _choice(_NORMS, kind, "kind")
+        if pre_weight is None:
+            raise N.GlinerDecideError(N.GD_ERR_INVALID_ARGUMENT, "pre_weight is needed")
+        pre_w, pre_b = _vector(pre_weight, y, C, "pre_weight"), _vector(pre_bias, y, C, "pre_bias")
+        post_w, post_b = _vector(post_weight, y, C, "post_weight"), _vector(post_bias, y, C, "post_bias")
+        y2, r2 = _rows2(y, C), _rows2(residual, C)
+        rows = y2.shape[0]
+        g, per_gate = N.GdRows(None, 0), 1
+        if gate is not None:
+            same_kind(gate, y, "gate")
+            g2, per_gate = self._gate_rows(gate, shape, rows)
+            g = N.GdRows(g2.data_ptr(), g2.stride(0) if g2.shape[0] > 1 else C)
+        if out is None:
+            h = torch.empty(shape, dtype=residual.dtype, device=y.device)
+            n = torch.empty(shape, dtype=y.dtype, device=y.device)
+            ldh = ldn = C
+        else:
+            h, n = out
+            _output(h, r2, shape, "out[0]")
+            _output(n, y2, shape, "out[1]")
+            ldh = h.stride(0) if h.dim() == 2 and rows > 1 else C
+            ldn = n.stride(0) if n.dim() == 2 and rows > 1 else C
+        call_on(y, self._lib.gd_block_norm, N.GdRows(y2.data_ptr(), y2.stride(0) if rows > 1 else C),
+                N.GdRows(r2.data_ptr(), r2.stride(0) if rows > 1 else C), g, per_gate, ptr(post_w), ptr(post_b),
+                ptr(pre_w), ptr(pre_b), h.data_ptr(), ldh, n.data_ptr(), ldn, rows, C, float(eps), float(scale), code,
+                dtype, N.GD_F32 if residual.dtype == torch.float32 else dtype)
+        return h, n
+
+    @staticmethod
+    def _gate_rows(gate: torch.Tensor, shape: tuple, rows: int):
+        """A gate that broadcasts to `shape` as [G, C] with row r's gate at r // (rows // G)."""
+        C = shape[-1]
+        lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape[:-1])
+        if gate.dim() < 1 or gate.dim() > len(shape) or gate.shape[-1] != C or any(
+                a not in (1, b) for a, b in zip(lead, shape[:-1])):
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"gate {tuple(gate.shape)} does not broadcast to {shape}")
+        n = math.prod(lead)
+        # its own leading axes first and broadcast ones behind: each gate row serves a run of rows
+        own = 0
+        while own < len(lead) and lead[own] == shape[own]:
+            own += 1
+        if any(d != 1 for d in lead[own:]):
+            gate = gate.expand(shape)
+            n = rows
+        return _rows2(gate.reshape(n, C) if gate.dim() != 2 or gate.shape[0] != n else gate, C), max(rows // max(n, 1), 1)
 
     def relative_index_table(self, n: int, device=None) -> torch.Tensor:
         """Device-computed idx(r) for r in [-(n-1), n-1] (DeBERTa.swift:521-551)."""

@@ -245,6 +245,101 @@ int gd_deberta_attention(gd_bhld q, gd_bhld k, gd_bhld v, gd_table pos_key, gd_t
                          int32_t bucket_size, int32_t output, void* out, int64_t ldo,
                          void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * One block over packed rows: attention with grouped heads, projections with
+ * a residual epilogue, the norms between two blocks.  No counterpart in the
+ * reference, whose graph is the encoder above.  `dtype` is GD_F16 or GD_BF16;
+ * sums, softmax statistics and norms are fp32, each output is rounded once.
+ * Forward only.
+ * ------------------------------------------------------------------------ */
+
+/* Packed tokens [T, H, D] with contiguous D: element (t, h, d) at
+ * data + t*stride_t + h*stride_h + d. */
+typedef struct gd_tokens {
+  const void* data;
+  int64_t stride_t, stride_h;
+} gd_tokens;
+
+/* Rows [R, C] with contiguous C: element (r, c) at data + r*stride + c. */
+typedef struct gd_rows {
+  const void* data;
+  int64_t stride;
+} gd_rows;
+
+/* Flags of gd_packed_attention. */
+#define GD_PACKED_CAUSAL 1u     /* query i of a sequence of nq queries and nk keys sees the keys
+                                   j <= nk - nq + i (the last query sees every key); without
+                                   it every query sees every key of its sequence */
+#define GD_PACKED_ZERO_REST 2u  /* rows of `out` that belong to no sequence are set to 0;
+                                   without it they are left as they were */
+
+/* Softmax attention over packed sequences:
+ *   out[t, h, :] = sum_j exp(scale q_t,h . k_j,g) v_j,g / sum_j exp(scale q_t,h . k_j,g),
+ * g = h / (heads / kv_heads), j over the keys of t's sequence that it sees; a
+ * query that sees no key gets 0.  What a query does not see has no effect on
+ * it, infinities and NaN included.
+ * q [q_tokens, heads, head_dim], k and v [k_tokens, kv_heads, head_dim], out
+ * [q_tokens, heads, head_dim] with rows of ldo elements; out overlaps none of
+ * them.  Sequence b holds queries [q_offsets[b], q_offsets[b + 1]) and keys
+ * [k_offsets[b], k_offsets[b + 1]); both are device int32 arrays of batch + 1
+ * entries that do not decrease (k_offsets = NULL: the keys are the queries'
+ * own tokens; k_tokens = q_tokens then).  They are not checked: entries
+ * outside [0, tokens] are held to that range, and offsets that decrease give
+ * undefined rows but no access outside the tensors.
+ * heads is a multiple of kv_heads; head_dim is 32, 64, 96, 128, 192 or 256;
+ * strides are multiples of 8 elements, data 16-byte aligned; at most
+ * 2^31 - 1 tokens.  `workspace` (device, 16-byte aligned) lets few queries be
+ * split over their keys: gd_packed_attention_workspace gives the bytes for
+ * the same numbers (0 where no split would be made); NULL or fewer bytes make
+ * the call without a split.  Calls that may run at the same time need a
+ * workspace each. */
+int64_t gd_packed_attention_workspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int64_t heads,
+                                      int64_t kv_heads, int64_t head_dim);
+int gd_packed_attention(gd_tokens q, gd_tokens k, gd_tokens v, const int32_t* q_offsets,
+                        const int32_t* k_offsets, int64_t batch, int64_t q_tokens, int64_t k_tokens,
+                        int64_t heads, int64_t kv_heads, int64_t head_dim, int32_t dtype, float scale,
+                        uint32_t flags, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* Activations of gd_projection. */
+typedef enum gd_activation {
+  GD_ACT_NONE = 0,
+  GD_ACT_RELU = 1,
+  GD_ACT_GELU = 2,      /* x Phi(x), exact erf form */
+  GD_ACT_GELU_TANH = 3, /* its tanh form: 0.5 x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) */
+  GD_ACT_SILU = 4       /* x / (1 + exp(-x)) */
+} gd_activation;
+
+/* out[i, j] = residual[i, j] + scale * act(sum_c x[i, c] w[j, c] + bias[j]),
+ * rounded once.  x [m, k], w [n, k], bias [n] or NULL, residual [m, n] (data
+ * NULL: none), out [m, n].  Any m, n >= 0 and k >= 1 with every row stride at least the
+ * row's length; data aligned to its element (rows of 16-byte alignment and
+ * stride run faster).  out may be the residual itself (same data and stride);
+ * it overlaps nothing else. */
+int gd_projection(gd_rows x, gd_rows w, const void* bias, gd_rows residual, void* out, int64_t ldo,
+                  int64_t m, int64_t n, int64_t k, int32_t activation, float scale, int32_t dtype,
+                  void* stream);
+
+/* Norms of gd_block_norm. */
+#define GD_NORM_LAYER 0 /* (x - mean) rsqrt(var + eps) weight + bias, biased variance */
+#define GD_NORM_RMS 1   /* x rsqrt(mean(x^2) + eps) weight + bias */
+
+/* Between two blocks: the norm after a block, its gate and residual scale, and
+ * the norm before the next one, in one pass over the rows:
+ *   h = residual + scale * gate * post(y),   n = pre(h)
+ * post(y) = y where post_weight is NULL; gate = 1 where gate.data is NULL, else
+ * row r's gate is row r / rows_per_gate of `gate`.  pre() takes h before it is
+ * rounded.  y, gate, weights, biases and n have `dtype`, residual and h have
+ * `stream_dtype` (`dtype` or GD_F32); biases may be NULL.  rows of cols in
+ * [1, 32768] elements; data aligned to its element.  h may be the residual and
+ * n may be y (same data and stride; h may be y and n the residual where their
+ * types are one); otherwise h and n overlap nothing. */
+int gd_block_norm(gd_rows y, gd_rows residual, gd_rows gate, int64_t rows_per_gate,
+                  const void* post_weight, const void* post_bias, const void* pre_weight,
+                  const void* pre_bias, void* h, int64_t ldh, void* n, int64_t ldn, int64_t rows,
+                  int64_t cols, float eps, float scale, int32_t kind, int32_t dtype,
+                  int32_t stream_dtype, void* stream);
+
 /* Writes the kernel's relative index idx(r) = clip(bucket(r) + bucket_size,
  * 0, 2*bucket_size-1) for r in [-(n-1), n-1] to out[r + n - 1] (device int32,
  * 2n-1 entries).  Exposes the device bucket math for parity tests
