@@ -66,6 +66,7 @@ bool overlap(const ByteRows& a, const ByteRows& b) {
 }
 
 constexpr int64_t kMaxDim = 0x7fffffff;
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;
 // Row strides are held to 2^40 elements, so that no byte range overflows.
 constexpr int64_t kMaxStride = (int64_t)1 << 40;
 bool stride_ok(int64_t stride, int64_t cols, int64_t rows) {
@@ -288,7 +289,7 @@ int gd_deberta_attention(gd_bhld q, gd_bhld k, gd_bhld v, gd_table pos_key, gd_t
 int64_t gd_packed_attention_workspace(int64_t batch, int64_t q_tokens, int64_t k_tokens, int64_t heads,
                                       int64_t kv_heads, int64_t head_dim) {
   if (batch <= 0 || q_tokens <= 0 || k_tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  if (batch > kMaxDim || q_tokens > kMaxDim || k_tokens > kMaxDim || heads > 4096 || heads % kv_heads != 0 ||
+  if (batch > kMaxTokens || q_tokens > kMaxTokens || k_tokens > kMaxTokens || heads > 4096 || heads % kv_heads != 0 ||
       head_dim > 256)
     return 0;
   return packed_attention_workspace(batch, q_tokens, k_tokens, heads, kv_heads, head_dim);
@@ -302,9 +303,9 @@ int gd_packed_attention(gd_tokens q, gd_tokens k, gd_tokens v, const int32_t* q_
   GD_CHECK_ARG(dtype == GD_F16 || dtype == GD_BF16, "dtype must be GD_F16 or GD_BF16 (got %d)", dtype);
   GD_CHECK_ARG((flags & ~(GD_PACKED_CAUSAL | GD_PACKED_ZERO_REST)) == 0, "unknown flags 0x%x", flags);
   GD_CHECK_ARG(std::isfinite(scale), "scale must be finite");
-  GD_CHECK_SHAPE(batch >= 0 && q_tokens >= 0 && k_tokens >= 0 && batch < kMaxDim && q_tokens <= kMaxDim &&
-                     k_tokens <= kMaxDim,
-                 "batch and token counts must be in [0, 2^31)");
+  GD_CHECK_SHAPE(batch >= 0 && q_tokens >= 0 && k_tokens >= 0 && batch <= kMaxTokens && q_tokens <= kMaxTokens &&
+                     k_tokens <= kMaxTokens,
+                 "batch and token counts must be in [0, 2^30]");
   GD_CHECK_SHAPE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 4096,
                  "heads must be a positive multiple of kv_heads, at most 4096 (got %lld, %lld)", (long long)heads,
                  (long long)kv_heads);
@@ -312,17 +313,17 @@ int gd_packed_attention(gd_tokens q, gd_tokens k, gd_tokens v, const int32_t* q_
                      head_dim == 256,
                  "head_dim must be 32, 64, 96, 128, 192 or 256 (got %lld)", (long long)head_dim);
   GD_CHECK_SHAPE(k_offsets || k_tokens == q_tokens, "without k_offsets the keys are the queries' own tokens");
-  GD_CHECK_SHAPE(ldo >= heads * head_dim && ldo % 8 == 0 && ldo <= kMaxStride / (q_tokens + 1),
-                 "ldo must be a multiple of 8 and at least heads * head_dim");
+  GD_CHECK_SHAPE(ldo >= heads * head_dim && ldo % 8 == 0 && ldo < (1 << 24),
+                 "ldo must be a multiple of 8, at least heads * head_dim and below 2^24");
   const gd_tokens* views[3] = {&q, &k, &v};
   for (int i = 0; i < 3; ++i) {
     const gd_tokens* t = views[i];
-    const int64_t tokens = i == 0 ? q_tokens : k_tokens, nh = i == 0 ? heads : kv_heads;
+    const int64_t nh = i == 0 ? heads : kv_heads;
     GD_CHECK_ARG(aligned(t->data, 16) && t->stride_t % 8 == 0 && t->stride_h % 8 == 0,
                  "q/k/v must be 16-byte aligned with strides that are multiples of 8 elements");
-    GD_CHECK_SHAPE(t->stride_t >= 0 && t->stride_h >= 0 && t->stride_t <= kMaxStride / (tokens + 1) &&
+    GD_CHECK_SHAPE(t->stride_t >= 0 && t->stride_h >= 0 && t->stride_t < (1 << 24) &&
                        t->stride_h <= kMaxStride / nh,
-                   "q/k/v strides must not be negative");
+                   "q/k/v strides must not be negative, token strides below 2^24 elements");
   }
   if (q_tokens == 0) return GD_OK;
   GD_CHECK_ARG(q.data && q_offsets && out, "null tensor pointer");

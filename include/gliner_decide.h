@@ -287,8 +287,8 @@ typedef struct gd_rows {
  * outside [0, tokens] are held to that range, and offsets that decrease give
  * undefined rows but no access outside the tensors.
  * heads is a multiple of kv_heads; head_dim is 32, 64, 96, 128, 192 or 256;
- * strides are multiples of 8 elements, data 16-byte aligned; at most
- * 2^31 - 1 tokens.  `workspace` (device, 16-byte aligned) lets few queries be
+ * strides are multiples of 8 elements (those of tokens below 2^24), data
+ * 16-byte aligned; at most 2^30 tokens.  `workspace` (device, 16-byte aligned) lets few queries be
  * split over their keys: gd_packed_attention_workspace gives the bytes for
  * the same numbers (0 where no split would be made); NULL or fewer bytes make
  * the call without a split.  Calls that may run at the same time need a
