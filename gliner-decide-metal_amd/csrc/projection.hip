@@ -1,77 +1,492 @@
 // out = residual + scale * act(x w^T + bias), fp16 and bf16, any sizes.
+//
+// Sums are fp32 on the matrix cores (few rows: fp32 multiply-adds), the
+// epilogue works on them in fp32 and rounds once.  Kernels:
+//   * tile_kernel, many rows: a BM x BN tile of 32x32x16 MFMA sub-tiles, 64-wide
+//     K steps brought into LDS by DMA two stages deep (rows of 16-byte
+//     alignment) or through registers (any alignment), the tile staged through
+//     LDS in fp32 so that the epilogue loads the residual and stores the
+//     output in whole 16-byte pieces of rows;
+//   * strip_kernel, up to 64 rows: W is read once, straight from global memory
+//     into the MFMA operands; the waves of a workgroup share a strip of 16 or
+//     32 columns and split K;
+//   * row_kernel, up to 4 rows: a wave a column or two, lanes along K.
+#include <algorithm>
+
 #include "elem16.hpp"
 #include "gd_kernels.hpp"
 
 namespace gd {
 namespace {
 
-constexpr int kBM = 64, kBN = 64, kBK = 32;
+// 0.5 erfc(|y| / sqrt(2)) as t q(t) exp(-y^2 / 2), t = 1 / (1 + 0.51 |y| / sqrt(2)),
+// q a minimax fit of erfcx over [0, 10]: 9e-7 of its value everywhere, so GELU's
+// lower tail keeps its digits.
+__device__ __forceinline__ float half_erfc(float y) {
+  const float z = fabsf(y);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.51f * 0.70710678f, z, 1.0f));
+  float q = 0.04725245f;
+  q = fmaf(q, t, -0.17957604f);
+  q = fmaf(q, t, 0.17923456f);
+  q = fmaf(q, t, 0.02751835f);
+  q = fmaf(q, t, 0.13953599f);
+  q = fmaf(q, t, 0.14207563f);
+  q = fmaf(q, t, 0.14395879f);
+  return q * t * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+}
 
 template <int ACT>
 __device__ __forceinline__ float activate(float y) {
   if (ACT == GD_ACT_RELU) return y > 0.f ? y : (y <= 0.f ? 0.f : y);
-  if (ACT == GD_ACT_GELU) return 0.5f * y * erfcf(-0.70710678f * y);
-  if (ACT == GD_ACT_GELU_TANH) return y / (1.0f + expf(-1.5957691216f * (y + 0.044715f * y * y * y)));
-  if (ACT == GD_ACT_SILU) return y / (1.0f + expf(-y));
+  if (ACT == GD_ACT_GELU) {
+    const float h = half_erfc(y);
+    return y * (y < 0.f ? h : 1.0f - h);
+  }
+  // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2 u))
+  if (ACT == GD_ACT_GELU_TANH)
+    return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.30220820f * fmaf(0.044715f * y * y, y, y)));
+  if (ACT == GD_ACT_SILU) return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * y));
   return y;
 }
 
-// A 64 x 64 tile a workgroup of four waves, operands through LDS in steps of
-// 32 columns, each element loaded by itself.
-template <class T, int ACT>
-__global__ __launch_bounds__(256) void projection_kernel(ProjectionArgs a) {
-  __shared__ __attribute__((aligned(16))) T xs[kBM][kBK + 8];
-  __shared__ __attribute__((aligned(16))) T ws[kBN][kBK + 8];
+// Eight elements at any alignment of the type; n < 8: the first n, then zeros.
+template <class T>
+__device__ __forceinline__ typename Elem<T>::v8 load8(const T* p, int n = 8) {
+  typename Elem<T>::v8 r;
+  if (n >= 8) {
+    __builtin_memcpy(&r, p, 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = e < n ? p[e] : (T)0.f;
+  }
+  return r;
+}
+
+// Epilogue of N consecutive elements of a row from column col (those below n).
+template <class T, int ACT, int N>
+__device__ __forceinline__ void finish(const ProjectionArgs& a, int64_t row, int64_t col, const float* acc,
+                                       const float* bias) {
+  const T* res = a.residual ? (const T*)a.residual + row * a.ldr + col : nullptr;
+  T* out = (T*)a.out + row * a.ldo + col;
+  T r[N];
+  if (col + N <= a.n) {
+    if (res) __builtin_memcpy(r, res, 2 * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float y = a.scale * activate<ACT>(acc[e] + bias[e]);
+      r[e] = (T)(res ? y + (float)r[e] : y);
+    }
+    __builtin_memcpy(out, r, 2 * N);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (col + e < a.n) {
+        const float y = a.scale * activate<ACT>(acc[e] + bias[e]);
+        out[e] = (T)(res ? y + (float)res[e] : y);
+      }
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void load_bias(const ProjectionArgs& a, int64_t col, float* b) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) b[e] = a.bias && col + e < a.n ? (float)((const T*)a.bias)[col + e] : 0.f;
+}
+
+// ---------------------------------------------------------------------------
+// Many rows.
+// ---------------------------------------------------------------------------
+constexpr int kBK = 64;
+
+// LDS rows of 64 elements (128 bytes): 16-byte chunk c of row r at chunk
+// c ^ ((r / 2) & 7), so that the 16 rows of a fragment read at one chunk cover
+// the 64 banks.
+__device__ __forceinline__ int tile_offset(int row, int chunk) { return row * kBK + ((chunk ^ ((row >> 1) & 7)) << 3); }
+
+template <class T, int BM, int BN, int WAVES_M, int NW, int ACT, bool DMA>
+__global__ __launch_bounds__(64 * NW) void tile_kernel(ProjectionArgs a, int tiles_m, int tiles_n) {
   typedef typename Elem<T>::v8 v8;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int64_t tiles_n = (a.n + kBN - 1) / kBN;
-  const int64_t m0 = blockIdx.x / tiles_n * kBM, n0 = blockIdx.x % tiles_n * kBN;
-  float4_t acc[4] = {};
-  for (int64_t k0 = 0; k0 < a.k; k0 += kBK) {
-    for (int i = t; i < kBM * kBK; i += 256) {
-      const int r = i / kBK, c = i % kBK;
-      xs[r][c] = m0 + r < a.m && k0 + c < a.k ? ((const T*)a.x)[(m0 + r) * a.ldx + k0 + c] : (T)0.f;
-      ws[r][c] = n0 + r < a.n && k0 + c < a.k ? ((const T*)a.w)[(n0 + r) * a.ldw + k0 + c] : (T)0.f;
+  constexpr int NT = 64 * NW, WAVES_N = NW / WAVES_M;
+  constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 32, TN = WN / 32;
+  constexpr int A_IT = BM / 8 / NW, B_IT = BN / 8 / NW;  // 1 KiB DMA pieces (8 rows) a wave and stage
+  constexpr int STAGE = (BM + BN) * kBK;
+  constexpr int LPS = A_IT + B_IT;
+  static_assert(TM >= 1 && TN >= 1 && A_IT >= 1 && B_IT >= 1, "tile shape");
+  // (an array a stage, named at compile time: the compiler then waits for the
+  // stage being read and leaves the DMA into the other in flight)
+  __shared__ __attribute__((aligned(1024))) T st0[STAGE];
+  __shared__ __attribute__((aligned(1024))) T st1[STAGE];
+
+  // Tile order: workgroups go round the 8 XCDs; each XCD takes a run of the
+  // tiles in bands of four tile rows, whose x rows and w rows its L2 then serves.
+  const int nwg = tiles_m * tiles_n, xcd = blockIdx.x & 7;
+  const int bid = xcd * (nwg >> 3) + min(xcd, nwg & 7) + (blockIdx.x >> 3);
+  const int band = bid / (4 * tiles_n), in_band = bid - band * 4 * tiles_n;
+  const int gm = min(4, tiles_m - band * 4);
+  const int64_t m0 = (int64_t)(band * 4 + in_band % gm) * BM, n0 = (int64_t)(in_band / gm) * BN;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const int lr = lane & 31, lk = lane >> 5;
+  const int mrows = (int)min((int64_t)BM, a.m - m0), nrows = (int)min((int64_t)BN, a.n - n0);
+  const T* xt = (const T*)a.x + m0 * a.ldx;
+  const T* wt = (const T*)a.w + n0 * a.ldw;
+
+  float16_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  v8 fa[2][TM], fb[2][TN];
+  const int lane_row = lr * kBK, swz = (lr >> 1) & 7;
+  auto read_frags = [&](const T* st, int s, int set) {
+    const int lo = lane_row + (((2 * s + lk) ^ swz) << 3);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[set][i] = *reinterpret_cast<const v8*>(st + (wm * WM + i * 32) * kBK + lo);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[set][j] = *reinterpret_cast<const v8*>(st + (BM + wn * WN + j * 32) * kBK + lo);
+  };
+  // w rows are the A operand: a lane holds four consecutive columns of a row
+  auto mma = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = Elem<T>::mfma32(fb[set][j], fa[set][i], acc[i][j]);
+  };
+  // One MFMA, one fragment read, and so on: without an order the two fragment
+  // sets fold into one with a wait before each group of MFMAs.
+  auto interleave = [&]() {
+#pragma unroll
+    for (int r = 0; r < TM + TN; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    if constexpr (TM * TN > TM + TN) __builtin_amdgcn_sched_group_barrier(0x008, TM * TN - (TM + TN), 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step of fewer than 64 columns, or one of unaligned rows: pieces of eight
+  // elements through registers, zeros past the last column.
+  constexpr int PIECES = (BM + BN) * 8 / NT;
+  auto load_step = [&](int64_t k0, v8* r) {
+    const int left = (int)min((int64_t)kBK, a.k - k0);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int p = tid + i * NT, row = p >> 3, c = (p & 7) * 8;
+      const T* src = row < BM ? xt + min(row, mrows - 1) * a.ldx : wt + min(row - BM, nrows - 1) * a.ldw;
+      r[i] = load8(src + k0 + c, left - c);
+    }
+  };
+  auto store_step = [&](T* st, const v8* r) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int p = tid + i * NT;
+      *reinterpret_cast<v8*>(st + tile_offset(p >> 3, p & 7)) = r[i];
+    }
+  };
+  auto compute_step = [&](const T* st) {
+    read_frags(st, 0, 0);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (s < 3) read_frags(st, s + 1, (s + 1) & 1);
+      mma(s & 1);
+    }
+  };
+
+  if constexpr (DMA) {
+    const int steps = (int)(a.k / kBK);
+    // lane l of a piece brings the chunk that lands at chunk l % 8 of row l / 8
+    uint32_t a_off[A_IT], b_off[B_IT];
+#pragma unroll
+    for (int i = 0; i < A_IT; ++i) {
+      const int r = (wave * A_IT + i) * 8 + (lane >> 3);
+      a_off[i] = (uint32_t)(min(r, mrows - 1) * (uint32_t)a.ldx + (((lane & 7) ^ ((r >> 1) & 7)) << 3));
+    }
+#pragma unroll
+    for (int i = 0; i < B_IT; ++i) {
+      const int r = (wave * B_IT + i) * 8 + (lane >> 3);
+      b_off[i] = (uint32_t)(min(r, nrows - 1) * (uint32_t)a.ldw + (((lane & 7) ^ ((r >> 1) & 7)) << 3));
+    }
+    auto issue = [&](T* st, int step) {
+      const T* xs = xt + (int64_t)min(step, steps - 1) * kBK;
+      const T* ws = wt + (int64_t)min(step, steps - 1) * kBK;
+#pragma unroll
+      for (int i = 0; i < A_IT; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)(xs + a_off[i]), (lds_void_t*)(st + (wave * A_IT + i) * 512), 16,
+                                         0, 0);
+#pragma unroll
+      for (int i = 0; i < B_IT; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)(ws + b_off[i]),
+                                         (lds_void_t*)(st + BM * kBK + (wave * B_IT + i) * 512), 16, 0, 0);
+    };
+    // Every step issues one stage (past the last step that one again, which
+    // nobody reads), so each wait is for a constant number of loads.
+    auto step = [&](T* st, const T* next, int t) {
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        read_frags(st, s + 1, (s + 1) & 1);
+        mma(s & 1);
+        interleave();
+      }
+      wait_vmcnt<0>();
+      stage_barrier();  // the next stage has landed, this one is in everyone's registers
+      issue(st, t + 2);
+      read_frags(next, 0, 0);
+      mma(1);
+      interleave();
+    };
+    if (steps > 0) {
+      issue(st0, 0);
+      issue(st1, 1);
+      wait_vmcnt<LPS>();
+      stage_barrier();
+      read_frags(st0, 0, 0);
+      int t = 0;
+      for (; t + 2 <= steps; t += 2) {
+        step(st0, st1, t);
+        step(st1, st0, t + 1);
+      }
+      if (t < steps) step(st0, st1, t);
+      wait_vmcnt<0>();
+      __syncthreads();
+    }
+    if (a.k % kBK != 0) {
+      v8 r[PIECES];
+      load_step((int64_t)steps * kBK, r);
+      store_step(st0, r);
+      __syncthreads();
+      compute_step(st0);
+      __syncthreads();
+    }
+  } else {
+    const int64_t steps = (a.k + kBK - 1) / kBK;
+    v8 r[PIECES];
+    load_step(0, r);
+    for (int64_t t = 0; t < steps; ++t) {
+      store_step(st0, r);
+      __syncthreads();
+      if (t + 1 < steps) load_step((t + 1) * kBK, r);
+      compute_step(st0);
+      __syncthreads();
+    }
+  }
+
+  // ---- epilogue: the tile through LDS in fp32, 16-byte unit u of row r at
+  // u ^ (r & 15) (16 rows at one unit cover the banks), out in rows ----
+  constexpr int RP = STAGE / 2 / BN / 32 * 32;  // rows that a stage holds
+  constexpr int UPR = BN / 8;                   // pieces of eight columns a row
+  static_assert(RP >= 32 && NT % UPR == 0, "epilogue shape");
+  const int u = tid % UPR;
+  float bias[8];
+  load_bias<T, 8>(a, n0 + 8 * u, bias);
+#pragma unroll
+  for (int pass = 0; pass < (BM + 2 * RP - 1) / (2 * RP); ++pass) {
+    const int first = pass * 2 * RP;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int row0 = wm * WM + i * 32 - first;
+      if (row0 < 0 || row0 >= 2 * RP) continue;
+      float* dst = reinterpret_cast<float*>(row0 < RP ? st0 : st1) + (row0 % RP + lr) * BN;
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int unit = (wn * WN + j * 32) / 4 + 2 * q + lk;
+          *reinterpret_cast<float4_t*>(dst + 4 * (unit ^ (lr & 15))) =
+              (float4_t){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
     }
     __syncthreads();
-    const v8 fx = *(const v8*)&xs[16 * wave + (lane & 15)][8 * (lane >> 4)];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const v8 fw = *(const v8*)&ws[16 * j + (lane & 15)][8 * (lane >> 4)];
-      acc[j] = Elem<T>::mfma16(fw, fx, acc[j]);  // column of C: x row; rows of C: w rows
+    for (int r = tid / UPR; r < 2 * RP && first + r < mrows; r += NT / UPR) {
+      const float* src = reinterpret_cast<const float*>(r < RP ? st0 : st1) + (r < RP ? r : r - RP) * BN;
+      float v[8];
+      *reinterpret_cast<float4_t*>(v) = *reinterpret_cast<const float4_t*>(src + 4 * ((2 * u) ^ (r & 15)));
+      *reinterpret_cast<float4_t*>(v + 4) = *reinterpret_cast<const float4_t*>(src + 4 * ((2 * u + 1) ^ (r & 15)));
+      finish<T, ACT, 8>(a, m0 + first + r, n0 + 8 * u, v, bias);
     }
     __syncthreads();
   }
-  const int64_t row = m0 + 16 * wave + (lane & 15);
-  if (row >= a.m) return;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: 16 RB rows of x against a strip of 16 columns (rows of w); the NW
+// waves take every NW-th 32-wide step of K.  Operands come from global memory
+// as they are (x from the L2).  Rows past the last repeat it.
+// ---------------------------------------------------------------------------
+template <class T, int RB, int NW, int ACT>
+__global__ __launch_bounds__(64 * NW) void strip_kernel(ProjectionArgs a) {
+  typedef typename Elem<T>::v8 v8;
+  __shared__ float part[NW][16 * RB][17];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lc = lane & 15, lg = lane >> 4;
+  const int64_t n0 = blockIdx.x * (int64_t)16, m0 = blockIdx.y * (int64_t)(16 * RB);
+  const T* w = (const T*)a.w + min(n0 + lc, a.n - 1) * a.ldw;
+  const T* x[RB];
+  float4_t acc[RB];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int b = 0; b < RB; ++b) {
+    x[b] = (const T*)a.x + min(m0 + 16 * b + lc, a.m - 1) * a.ldx;
+    acc[b] = (float4_t){0.f, 0.f, 0.f, 0.f};
+  }
+  const int64_t steps = a.k / 32;
+  constexpr int U = 4;  // steps in flight
+  int64_t t = wave;
+  for (; t + (U - 1) * NW < steps; t += U * NW) {
+    v8 fw[U], fx[U][RB];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t col = n0 + 16 * j + 4 * (lane >> 4) + e;
-      if (col >= a.n) continue;
-      float y = acc[j][e];
-      if (a.bias) y += (float)((const T*)a.bias)[col];
-      y = a.scale * activate<ACT>(y);
-      if (a.residual) y += (float)((const T*)a.residual)[row * a.ldr + col];
-      ((T*)a.out)[row * a.ldo + col] = (T)y;
+    for (int i = 0; i < U; ++i) {
+      const int64_t k = (t + i * NW) * 32 + 8 * lg;
+      fw[i] = load8(w + k);
+#pragma unroll
+      for (int b = 0; b < RB; ++b) fx[i][b] = load8(x[b] + k);
     }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int b = 0; b < RB; ++b) acc[b] = Elem<T>::mfma16(fw[i], fx[i][b], acc[b]);
+  }
+  for (; t * 32 < a.k; t += NW) {
+    const int64_t k = t * 32 + 8 * lg;
+    const int left = (int)max(min(a.k - k, (int64_t)8), (int64_t)0);
+    const v8 fw = load8(w + k, left);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) acc[b] = Elem<T>::mfma16(fw, load8(x[b] + k, left), acc[b]);
+  }
+  // lane: row of x lc, columns 4 lg + e
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][16 * b + lc][4 * lg + e] = acc[b][e];
+  __syncthreads();
+  for (int i = tid; i < 16 * RB * 16; i += 64 * NW) {
+    const int r = i >> 4, c = i & 15;
+    if (m0 + r >= a.m || n0 + c >= a.n) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int j = 0; j < NW; ++j) v += part[j][r][c];
+    float bias;
+    load_bias<T, 1>(a, n0 + c, &bias);
+    finish<T, ACT, 1>(a, m0 + r, n0 + c, &v, &bias);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Up to four rows: a wave C columns, 64 lanes x 8 elements of K a step.
+// ---------------------------------------------------------------------------
+template <class T, int M, int C, int ACT>
+__global__ __launch_bounds__(256) void row_kernel(ProjectionArgs a) {
+  typedef typename Elem<T>::v8 v8;
+  const int lane = threadIdx.x & 63;
+  const int64_t n0 = (blockIdx.x * (int64_t)4 + (threadIdx.x >> 6)) * C;
+  if (n0 >= a.n) return;
+  const T* x = (const T*)a.x;
+  const T* w[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) w[c] = (const T*)a.w + min(n0 + c, a.n - 1) * a.ldw;
+  float acc[M][C] = {};
+  auto add = [&](const v8* fw, const v8* fx) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[m][c] = fmaf((float)fw[c][e], (float)fx[m][e], acc[m][c]);
+  };
+  int64_t k = lane * 8;
+  for (; k + 512 + 8 <= a.k; k += 1024) {
+    v8 fw[2][C], fx[2][M];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) fw[i][c] = load8(w[c] + k + 512 * i);
+#pragma unroll
+      for (int m = 0; m < M; ++m) fx[i][m] = load8(x + min((int64_t)m, a.m - 1) * a.ldx + k + 512 * i);
+    }
+    add(fw[0], fx[0]);
+    add(fw[1], fx[1]);
+  }
+  for (; k < a.k; k += 512) {
+    const int left = (int)min(a.k - k, (int64_t)8);
+    v8 fw[C], fx[M];
+#pragma unroll
+    for (int c = 0; c < C; ++c) fw[c] = load8(w[c] + k, left);
+#pragma unroll
+    for (int m = 0; m < M; ++m) fx[m] = load8(x + min((int64_t)m, a.m - 1) * a.ldx + k, left);
+    add(fw, fx);
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float v = wave_sum_dpp(acc[m][c]);
+      if (lane == m * C + c && m < a.m && n0 + c < a.n) {
+        float bias;
+        load_bias<T, 1>(a, n0 + c, &bias);
+        finish<T, ACT, 1>(a, m, n0 + c, &v, &bias);
+      }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+template <class T, int BM, int BN, int WAVES_M, int NW, int ACT, bool DMA>
+int launch_tile(const ProjectionArgs& a, hipStream_t stream) {
+  const int64_t tm = (a.m + BM - 1) / BM, tn = (a.n + BN - 1) / BN;
+  if (tm * tn > 0x7fffffff || tn > 0x1fffffff) return fail(GD_ERR_SHAPE, "projection: too many tiles");
+  tile_kernel<T, BM, BN, WAVES_M, NW, ACT, DMA>
+      <<<dim3((unsigned)(tm * tn)), dim3(64 * NW), 0, stream>>>(a, (int)tm, (int)tn);
+  GD_LAUNCH_CHECK();
+  return GD_OK;
+}
+
+template <class T, int ACT>
+int launch_act(const ProjectionArgs& a, hipStream_t stream) {
+  if (a.m <= 4) {
+    const int64_t blocks = (a.n + 3) / 4;
+    if (a.m == 1)
+      row_kernel<T, 1, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
+    else if (a.m == 2)
+      row_kernel<T, 2, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
+    else
+      row_kernel<T, 4, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
+    GD_LAUNCH_CHECK();
+    return GD_OK;
+  }
+  if (a.m <= 64) {
+    const int64_t strips = (a.n + 15) / 16;
+    const dim3 grid((unsigned)strips, 1);
+    if (a.m <= 16)
+      strip_kernel<T, 1, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
+    else if (a.m <= 32)
+      strip_kernel<T, 2, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
+    else
+      strip_kernel<T, 4, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
+    GD_LAUNCH_CHECK();
+    return GD_OK;
+  }
+  // DMA needs rows of 16-byte pieces and tile offsets within 32 bits
+  auto rows16 = [](const void* p, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 23);
+  };
+  if (!rows16(a.x, a.ldx) || !rows16(a.w, a.ldw)) return launch_tile<T, 128, 128, 2, 4, ACT, false>(a, stream);
+  const int64_t cus = device_cu_count();
+  auto tiles = [&](int bm, int bn) { return (a.m + bm - 1) / bm * ((a.n + bn - 1) / bn); };
+  if (tiles(256, 256) >= cus) return launch_tile<T, 256, 256, 2, 8, ACT, true>(a, stream);
+  if (tiles(128, 128) >= cus) return launch_tile<T, 128, 128, 2, 4, ACT, true>(a, stream);
+  return launch_tile<T, 64, 64, 2, 4, ACT, true>(a, stream);
 }
 
 template <class T>
 int launch(const ProjectionArgs& a, hipStream_t stream) {
-  const int64_t tiles = (a.m + kBM - 1) / kBM * ((a.n + kBN - 1) / kBN);
-  if (tiles > 0x7fffffff) return fail(GD_ERR_SHAPE, "projection: too many tiles");
-  const dim3 grid((unsigned)tiles), block(256);
   switch (a.activation) {
-    case GD_ACT_RELU: projection_kernel<T, GD_ACT_RELU><<<grid, block, 0, stream>>>(a); break;
-    case GD_ACT_GELU: projection_kernel<T, GD_ACT_GELU><<<grid, block, 0, stream>>>(a); break;
-    case GD_ACT_GELU_TANH: projection_kernel<T, GD_ACT_GELU_TANH><<<grid, block, 0, stream>>>(a); break;
-    case GD_ACT_SILU: projection_kernel<T, GD_ACT_SILU><<<grid, block, 0, stream>>>(a); break;
-    default: projection_kernel<T, GD_ACT_NONE><<<grid, block, 0, stream>>>(a);
+    case GD_ACT_RELU: return launch_act<T, GD_ACT_RELU>(a, stream);
+    case GD_ACT_GELU: return launch_act<T, GD_ACT_GELU>(a, stream);
+    case GD_ACT_GELU_TANH: return launch_act<T, GD_ACT_GELU_TANH>(a, stream);
+    case GD_ACT_SILU: return launch_act<T, GD_ACT_SILU>(a, stream);
+    default: return launch_act<T, GD_ACT_NONE>(a, stream);
   }
-  GD_LAUNCH_CHECK();
-  return GD_OK;
 }
 
 }  // namespace
