@@ -76,18 +76,20 @@ def dtype16(t: torch.Tensor, name: str) -> int:
 def same_kind(t: torch.Tensor, like: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> None:
     """Refuses a tensor on another device than `like`, or of another type than
     `dtype` (None: that of `like`)."""
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{name} must be on {like.device} (got {t.device})")
     dtype = dtype or like.dtype
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
 
 
 def call_on(t: torch.Tensor, fn, *args) -> None:
     """fn(*args, current stream) on t's device, whichever device is current."""
-    index = t.device.index
+    index = t.get_device()
     if index == _current_device():
-        N.check(fn(*args, stream_handle()))
+        status = fn(*args, stream_handle())
     else:
         with torch.cuda.device(index):
-            N.check(fn(*args, stream_handle()))
+            status = fn(*args, stream_handle())
+    if status != N.GD_OK:
+        N.check(status)

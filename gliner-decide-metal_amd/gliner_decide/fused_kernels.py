@@ -71,33 +71,41 @@ def _tokens(t: torch.Tensor, name: str) -> N.GdTokens:
     return N.GdTokens(t.data_ptr(), st if T > 1 else 0, sh if H > 1 else 0)
 
 
-def _rows2(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """[rows, cols] of any leading axes with contiguous, non-overlapping rows (copied where t has none)."""
-    if t.dim() != 2:
-        t = t.reshape(-1, cols) if cols else t.reshape(math.prod(t.shape[:-1]), 0)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+def _rows(t: torch.Tensor, cols: int):
+    """(tensor, GdRows) of t [..., cols] as rows with contiguous, non-overlapping columns (copied where t has none)."""
+    if not t.is_contiguous():
+        if t.dim() != 2:
+            t = t.reshape(-1, cols) if cols else t.reshape(math.prod(t.shape[:-1]), 0)
+        many = t.shape[0] > 1
+        if (cols <= 1 or t.stride(1) == 1) and (not many or t.stride(0) >= cols):
+            return t, N.GdRows(t.data_ptr(), t.stride(0) if many else cols)
         t = t.contiguous()
-    return t
+    return t, N.GdRows(t.data_ptr(), cols)
 
 
-def _vector(t: torch.Tensor | None, like: torch.Tensor, n: int, name: str) -> torch.Tensor | None:
+def _vector(t: torch.Tensor | None, like: torch.Tensor, shape: tuple, name: str) -> torch.Tensor | None:
     if t is None:
         return None
     same_kind(t, like, name)
-    if t.dim() != 1 or t.shape[0] != n:
-        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be [{n}] (got {tuple(t.shape)})")
+    if t.shape != shape:
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be {list(shape)} (got {tuple(t.shape)})")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _output(out: torch.Tensor, like: torch.Tensor, shape: tuple, name: str) -> None:
-    """Refuses a given output whose rows (last axis) are not contiguous at one row stride."""
+def _data(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _output(out: torch.Tensor, like: torch.Tensor, shape, name: str) -> int:
+    """Row stride of a given output; refuses one whose rows (last axis) are not contiguous at one stride."""
     same_kind(out, like, name)
-    if tuple(out.shape) != shape:
-        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be {shape} (got {tuple(out.shape)})")
-    if out.numel() and out.dim() != 2 and not out.is_contiguous():
+    if out.shape != shape:
+        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be {tuple(shape)} (got {tuple(out.shape)})")
+    if out.is_contiguous():
+        return shape[-1]
+    if out.dim() != 2 or (out.shape[1] > 1 and out.stride(1) != 1):
         raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be contiguous, or rows with contiguous columns")
-    if out.dim() == 2 and out.shape[1] > 1 and out.stride(1) != 1:
-        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must have contiguous columns")
+    return out.stride(0) if out.shape[0] > 1 else shape[-1]
 
 
 class FusedKernels:
@@ -297,10 +305,8 @@ class FusedKernels:
             ldo = out.stride(0) if Tq > 1 else H * D
         need = self._lib.gd_packed_attention_workspace(batch, Tq, Tk, H, Hk, D)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        call_on(q, self._lib.gd_packed_attention, qt, kt, vt, q_offsets.data_ptr(),
-                None if k_offsets is None else k_offsets.data_ptr(), batch, Tq, Tk, H, Hk, D, dtype,
-                D ** -0.5 if scale is None else float(scale), flags, out.data_ptr(), ldo,
-                None if work is None else work.data_ptr(), need)
+        call_on(q, self._lib.gd_packed_attention, qt, kt, vt, q_offsets.data_ptr(), _data(k_offsets), batch, Tq, Tk, H,
+                Hk, D, dtype, D ** -0.5 if scale is None else float(scale), flags, out.data_ptr(), ldo, _data(work), need)
         return out
 
     @staticmethod
@@ -326,26 +332,23 @@ class FusedKernels:
         if x.dim() < 1 or x.shape[-1] != K:
             raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"x {tuple(x.shape)} does not end in the weight's {K} columns")
         act = _choice(_ACTIVATIONS, activation, "activation")
-        shape = tuple(x.shape[:-1]) + (n,)
-        x2, w = _rows2(x, K), _rows2(weight, K)
-        m = x2.shape[0]
-        bias = _vector(bias, x, n, "bias")
+        shape = x.shape[:-1] + (n,)
+        x2, xr = _rows(x, K)
+        w2, wr = _rows(weight, K)
+        bias = _vector(bias, x, (n,), "bias")
         res = N.GdRows(None, 0)
         if residual is not None:
             same_kind(residual, x, "residual")
-            if tuple(residual.shape) != shape:
-                raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"residual must be {shape} (got {tuple(residual.shape)})")
-            r2 = _rows2(residual, n)
-            res = N.GdRows(r2.data_ptr(), r2.stride(0) if m > 1 else n)
+            if residual.shape != shape:
+                raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"residual must be {tuple(shape)} (got "
+                                                          f"{tuple(residual.shape)})")
+            residual, res = _rows(residual, n)
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
-            ldo = n
+            out, ldo = torch.empty(shape, dtype=x.dtype, device=x.device), n
         else:
-            _output(out, x, shape, "out")
-            ldo = out.stride(0) if out.dim() == 2 and m > 1 else n
-        call_on(x, self._lib.gd_projection, N.GdRows(x2.data_ptr(), x2.stride(0) if m > 1 else K),
-                N.GdRows(w.data_ptr(), w.stride(0) if n > 1 else K), None if bias is None else bias.data_ptr(), res,
-                out.data_ptr(), ldo, m, n, K, act, float(scale), dtype)
+            ldo = _output(out, x, shape, "out")
+        call_on(x, self._lib.gd_projection, xr, wr, _data(bias), res, out.data_ptr(), ldo,
+                x.numel() // K if K else 0, n, K, act, float(scale), dtype)
         return out
 
     def block_norm(self, y, residual, *, pre_weight, pre_bias=None, post_weight=None, post_bias=None, gate=None,
@@ -360,56 +363,59 @@ class FusedKernels:
         broadcasts to y's and keeps C ([C], [B, 1, C] for [B, L, C], y's own).
         out = (h, n) may be the residual and y themselves.  Forward only."""
         dtype = dtype16(y, "y")
-        same_kind(residual, y, "residual", torch.float32 if residual.dtype == torch.float32 else None)
-        if y.dim() < 1 or y.shape != residual.shape:
-            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"y {tuple(y.shape)} and residual {tuple(residual.shape)} differ")
-        C = y.shape[-1]
-        shape = tuple(y.shape)
+        f32 = residual.dtype is torch.float32
+        same_kind(residual, y, "residual", torch.float32 if f32 else None)
+        shape = y.shape
+        if y.dim() < 1 or residual.shape != shape:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"y {tuple(shape)} and residual {tuple(residual.shape)} differ")
+        C = shape[-1]
+        rows = y.numel() // C if C else 0
         code = _choice(_NORMS, kind, "kind")
         if pre_weight is None:
             raise N.GlinerDecideError(N.GD_ERR_INVALID_ARGUMENT, "pre_weight is needed")
-        pre_w, pre_b = _vector(pre_weight, y, C, "pre_weight"), _vector(pre_bias, y, C, "pre_bias")
-        post_w, post_b = _vector(post_weight, y, C, "post_weight"), _vector(post_bias, y, C, "post_bias")
-        y2, r2 = _rows2(y, C), _rows2(residual, C)
-        rows = y2.shape[0]
+        vec = (C,)
+        pre_w, pre_b = _vector(pre_weight, y, vec, "pre_weight"), _vector(pre_bias, y, vec, "pre_bias")
+        post_w, post_b = _vector(post_weight, y, vec, "post_weight"), _vector(post_bias, y, vec, "post_bias")
+        y2, yr = _rows(y, C)
+        r2, rr = _rows(residual, C)
         g, per_gate = N.GdRows(None, 0), 1
         if gate is not None:
             same_kind(gate, y, "gate")
-            g2, per_gate = self._gate_rows(gate, shape, rows)
-            g = N.GdRows(g2.data_ptr(), g2.stride(0) if g2.shape[0] > 1 else C)
+            gate, per_gate = self._gate_rows(gate, shape, rows)
+            gate, g = _rows(gate, C)
         if out is None:
             h = torch.empty(shape, dtype=residual.dtype, device=y.device)
             n = torch.empty(shape, dtype=y.dtype, device=y.device)
             ldh = ldn = C
         else:
             h, n = out
-            _output(h, r2, shape, "out[0]")
-            _output(n, y2, shape, "out[1]")
-            ldh = h.stride(0) if h.dim() == 2 and rows > 1 else C
-            ldn = n.stride(0) if n.dim() == 2 and rows > 1 else C
-        call_on(y, self._lib.gd_block_norm, N.GdRows(y2.data_ptr(), y2.stride(0) if rows > 1 else C),
-                N.GdRows(r2.data_ptr(), r2.stride(0) if rows > 1 else C), g, per_gate, ptr(post_w), ptr(post_b),
-                ptr(pre_w), ptr(pre_b), h.data_ptr(), ldh, n.data_ptr(), ldn, rows, C, float(eps), float(scale), code,
-                dtype, N.GD_F32 if residual.dtype == torch.float32 else dtype)
+            ldh, ldn = _output(h, r2, shape, "out[0]"), _output(n, y2, shape, "out[1]")
+        call_on(y, self._lib.gd_block_norm, yr, rr, g, per_gate, _data(post_w), _data(post_b), _data(pre_w), _data(pre_b),
+                h.data_ptr(), ldh, n.data_ptr(), ldn, rows, C, float(eps), float(scale), code, dtype,
+                N.GD_F32 if f32 else dtype)
         return h, n
 
     @staticmethod
-    def _gate_rows(gate: torch.Tensor, shape: tuple, rows: int):
-        """A gate that broadcasts to `shape` as [G, C] with row r's gate at r // (rows // G)."""
+    def _gate_rows(gate: torch.Tensor, shape, rows: int):
+        """A gate that broadcasts to `shape`, as G rows of its last axis with row r's gate at r // (rows // G), and
+        rows // G."""
+        if gate.shape == shape:
+            return gate, 1
         C = shape[-1]
+        if gate.dim() < 1 or gate.dim() > len(shape) or gate.shape[-1] != C:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
+        if gate.dim() == 1:
+            return gate, max(rows, 1)
         lead = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape[:-1])
-        if gate.dim() < 1 or gate.dim() > len(shape) or gate.shape[-1] != C or any(
-                a not in (1, b) for a, b in zip(lead, shape[:-1])):
-            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"gate {tuple(gate.shape)} does not broadcast to {shape}")
-        n = math.prod(lead)
+        if any(a not in (1, b) for a, b in zip(lead, shape[:-1])):
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
         # its own leading axes first and broadcast ones behind: each gate row serves a run of rows
         own = 0
         while own < len(lead) and lead[own] == shape[own]:
             own += 1
         if any(d != 1 for d in lead[own:]):
-            gate = gate.expand(shape)
-            n = rows
-        return _rows2(gate.reshape(n, C) if gate.dim() != 2 or gate.shape[0] != n else gate, C), max(rows // max(n, 1), 1)
+            return gate.expand(shape), 1
+        return gate.reshape(-1, C), max(rows // max(math.prod(lead), 1), 1)
 
     def relative_index_table(self, n: int, device=None) -> torch.Tensor:
         """Device-computed idx(r) for r in [-(n-1), n-1] (DeBERTa.swift:521-551)."""
