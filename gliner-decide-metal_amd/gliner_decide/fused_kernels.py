@@ -63,12 +63,13 @@ def _choice(table: dict, key, name: str) -> int:
 
 def _tokens(t: torch.Tensor, name: str) -> N.GdTokens:
     """[T, H, D] with contiguous D; a stride that no element uses is 0."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
-        raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be a [tokens, heads, head_dim] view with contiguous "
-                                                  f"head_dim (got {tuple(t.shape)}, strides {t.stride()})")
-    T, H, _ = t.shape
-    st, sh, _ = t.stride()
-    return N.GdTokens(t.data_ptr(), st if T > 1 else 0, sh if H > 1 else 0)
+    if t.dim() == 3:
+        T, H, D = t.shape
+        st, sh, sd = t.stride()
+        if sd == 1 or D <= 1:
+            return N.GdTokens(t.data_ptr(), st if T > 1 else 0, sh if H > 1 else 0)
+    raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be a [tokens, heads, head_dim] view with contiguous "
+                                              f"head_dim (got {tuple(t.shape)}, strides {t.stride()})")
 
 
 def _rows(t: torch.Tensor, cols: int):
@@ -86,10 +87,12 @@ def _rows(t: torch.Tensor, cols: int):
 def _vector(t: torch.Tensor | None, like: torch.Tensor, shape: tuple, name: str) -> torch.Tensor | None:
     if t is None:
         return None
+    if t.dtype is like.dtype and t.get_device() == like.get_device() and t.shape == shape and t.is_contiguous():
+        return t
     same_kind(t, like, name)
     if t.shape != shape:
         raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be {list(shape)} (got {tuple(t.shape)})")
-    return t if t.is_contiguous() else t.contiguous()
+    return t.contiguous()
 
 
 def _data(t: torch.Tensor | None):
@@ -295,7 +298,7 @@ class FusedKernels:
                 raise N.GlinerDecideError(N.GD_ERR_SHAPE, "q_offsets and k_offsets must have one length")
         flags = N.GD_PACKED_CAUSAL if causal else 0
         if out is None:
-            out = torch.empty((Tq, H, D), dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ldo = H * D
             flags |= N.GD_PACKED_ZERO_REST
         else:
@@ -306,14 +309,15 @@ class FusedKernels:
         need = self._lib.gd_packed_attention_workspace(batch, Tq, Tk, H, Hk, D)
         work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         call_on(q, self._lib.gd_packed_attention, qt, kt, vt, q_offsets.data_ptr(), _data(k_offsets), batch, Tq, Tk, H,
-                Hk, D, dtype, D ** -0.5 if scale is None else float(scale), flags, out.data_ptr(), ldo, _data(work), need)
+                Hk, D, dtype, D ** -0.5 if scale is None else scale, flags, out.data_ptr(), ldo, _data(work), need)
         return out
 
     @staticmethod
     def _offsets(t: torch.Tensor, like: torch.Tensor, name: str):
-        if t.device != like.device:
+        if t.get_device() != like.get_device():
             raise ValueError(f"{name} must be on {like.device} (got {t.device})")
-        t = as_i32(t, name)
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            t = as_i32(t, name)
         if t.dim() != 1 or t.shape[0] < 1:
             raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be [batch + 1] (got {tuple(t.shape)})")
         return t, t.shape[0] - 1
@@ -384,8 +388,8 @@ class FusedKernels:
             gate, per_gate = self._gate_rows(gate, shape, rows)
             gate, g = _rows(gate, C)
         if out is None:
-            h = torch.empty(shape, dtype=residual.dtype, device=y.device)
-            n = torch.empty(shape, dtype=y.dtype, device=y.device)
+            h = torch.empty_like(residual, memory_format=torch.contiguous_format)
+            n = torch.empty_like(y, memory_format=torch.contiguous_format)
             ldh = ldn = C
         else:
             h, n = out
