@@ -40,23 +40,51 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ int clamp_to(int v, int hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
 
-// Sequence of a slot: the last i in [0, B] whose first slot, floor(off[i] * mul /
-// unit) + i, is at or before it; -1 before the first, B behind the last
-// sequence.  `first` is set to the found sequence's first slot (0 for -1).
-__device__ __forceinline__ int sequence_of_slot(const int32_t* off, int B, int tokens, int64_t mul, int unit,
-                                                int64_t slot, int64_t& first) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  first = 0;
-  for (int i0 = 0; i0 <= B; i0 += 64) {
+struct Sequence {
+  int q0, nq, k0, nk;
+};
+__device__ __forceinline__ Sequence sequence_of_offsets(const PackedAttentionArgs& a, int q0, int q1, int k0, int k1) {
+  Sequence r;
+  r.q0 = clamp_to(q0, (int)a.Tq);
+  r.nq = max(clamp_to(q1, (int)a.Tq) - r.q0, 0);
+  r.k0 = clamp_to(k0, (int)a.Tk);
+  r.nk = max(clamp_to(k1, (int)a.Tk) - r.k0, 0);
+  return r;
+}
+__device__ __forceinline__ Sequence sequence_at(const PackedAttentionArgs& a, int s) {
+  return sequence_of_offsets(a, a.q_off[s], a.q_off[s + 1], a.k_off[s], a.k_off[s + 1]);
+}
+
+// Sequence of a slot: the last i in [0, B] whose first slot, units(offset i) + i,
+// is at or before it; -1 before the first, B behind the last sequence (sq is
+// set for the others).  `first` is the found sequence's first slot (0 for -1).
+// Its offsets come from the lanes that looked: one trip to memory.
+template <bool BY_KEYS, class Units>
+__device__ __forceinline__ int sequence_of_slot(const PackedAttentionArgs& a, int64_t slot, Units units, int64_t& first,
+                                                Sequence& sq) {
+  const int lane = threadIdx.x & 63, B = (int)a.B;
+  for (int i0 = 0;; i0 += 64) {
     const int i = i0 + lane;
-    const int64_t start = i <= B ? clamp_to(off[i], tokens) * mul / unit + i : INT64_MAX;
+    const int qo = i <= B ? a.q_off[i] : 0, ko = i <= B ? a.k_off[i] : 0;
+    const int64_t start = i <= B ? units(clamp_to(BY_KEYS ? ko : qo, (int)(BY_KEYS ? a.Tk : a.Tq))) + i : INT64_MAX;
     const int c = __popcll(__ballot(start <= slot));
-    n += c;
-    if (c < 64) break;
+    if (c == 64 && i0 + 64 <= B) continue;
+    const int s = i0 + c - 1;
+    if (s < 0) {
+      first = 0;
+      return -1;
+    }
+    if (c > 0 && c < 64) {
+      const int q0 = __builtin_amdgcn_readlane(qo, c - 1), q1 = __builtin_amdgcn_readlane(qo, c);
+      const int k0 = __builtin_amdgcn_readlane(ko, c - 1), k1 = __builtin_amdgcn_readlane(ko, c);
+      first = units(clamp_to(BY_KEYS ? k0 : q0, (int)(BY_KEYS ? a.Tk : a.Tq))) + s;
+      if (s < B) sq = sequence_of_offsets(a, q0, q1, k0, k1);
+    } else {  // (this and the next offset lie in two rounds)
+      first = units(clamp_to(BY_KEYS ? a.k_off[s] : a.q_off[s], (int)(BY_KEYS ? a.Tk : a.Tq))) + s;
+      if (s < B) sq = sequence_at(a, s);
+    }
+    return s;
   }
-  if (n > 0) first = clamp_to(off[n - 1], tokens) * mul / unit + (n - 1);
-  return n - 1;
 }
 
 // Sequence of a token: the last i with off[i] <= t, in [-1, B].
@@ -71,26 +99,13 @@ __device__ __forceinline__ int sequence_of_token(const int32_t* off, int B, int 
   return n - 1;
 }
 
-struct Sequence {
-  int q0, nq, k0, nk;
-};
-__device__ __forceinline__ Sequence sequence_at(const PackedAttentionArgs& a, int s) {
-  Sequence r;
-  r.q0 = clamp_to(a.q_off[s], (int)a.Tq);
-  r.nq = max(clamp_to(a.q_off[s + 1], (int)a.Tq) - r.q0, 0);
-  r.k0 = clamp_to(a.k_off[s], (int)a.Tk);
-  r.nk = max(clamp_to(a.k_off[s + 1], (int)a.Tk) - r.k0, 0);
-  return r;
-}
-
 // What the host chooses for a call from its numbers alone.
 struct Plan {
-  int rb = 0;            // token_kernel's row blocks of 16 (0: it does not run)
-  bool prompt = false;   // prompt_kernel runs
-  int split = 1;         // its parts of the keys
-  int chunk = 0;         // token_kernel's keys a workgroup
-  int64_t k_slots = 0;   // its chunk slots
-  int64_t token_floats = 0, prompt_floats = 0;  // workspace of each, in floats
+  int rb = 0;           // token_kernel's row blocks of 16; 0: prompt_kernel
+  int split = 1;        // prompt_kernel's largest number of parts of the keys
+  int chunk = 0;        // token_kernel's keys a workgroup
+  int64_t k_slots = 0;  // its chunk slots
+  int64_t floats = 0;   // workspace for the parts
 };
 
 // Workspace rows: D sums, then the running maximum (in units of log2) and sum.
@@ -204,12 +219,18 @@ __device__ __forceinline__ void zero_rows(const PackedAttentionArgs& a, int hk, 
   }
 }
 
+// Keys of a part where a tile of the prompt kernel sees `seen` keys and has
+// room for `split` parts: whole steps, at least four.
+__device__ __forceinline__ int part_keys(int seen, int split) {
+  return split == 1 ? INT_MAX / 64 * 64 : max(((seen + split - 1) / split + 63) / 64 * 64, 256);
+}
+
 // ---------------------------------------------------------------------------
 // Many rows a sequence.
 // ---------------------------------------------------------------------------
 template <class T, int D, int NW, bool CAUSAL>
 __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(PackedAttentionArgs a, int G, int Hk, int slots, int split,
-                                                            int small_rows, float* parts) {
+                                                            float* parts) {
   typedef typename Elem<T>::v8 v8;
   typedef typename Elem<T>::v4 v4;
   constexpr int BM = 32 * NW, KT = 64, DP = padded(D);
@@ -234,7 +255,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
   const int64_t slot = slots - 1 - idx / split;
   int64_t first;
   // (one more slot in front: rows before the first sequence)
-  const int s = slot == 0 ? -1 : sequence_of_slot(a.q_off, (int)a.B, (int)a.Tq, G, BM, slot - 1, first);
+  Sequence sq;
+  const int s = slot == 0 ? -1
+                          : sequence_of_slot<false>(a, slot - 1, [&](int o) { return (int64_t)o * G / BM; }, first, sq);
   const int tid = threadIdx.x;
   if (s < 0 || s >= a.B) {
     if (a.zero_rest && part == 0) {
@@ -248,10 +271,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
     }
     return;
   }
-  const Sequence sq = sequence_at(a, s);
   const int64_t rows = (int64_t)sq.nq * G;
   const int64_t row0 = (slot - 1 - first) * BM;
-  if (row0 >= rows || rows <= small_rows) return;
+  if (row0 >= rows) return;
 
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, lh = lane >> 5;
@@ -271,9 +293,16 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
   const int seen_min = CAUSAL ? max(min(shift + (int)tok_first + 1, sq.nk), 0) : sq.nk;
   const int seen_max = CAUSAL ? max(min(shift + tok_end + 1, sq.nk), 0) : sq.nk;
   const int tiles_all = (seen_max + KT - 1) / KT;
-  const int per = (tiles_all + split - 1) / split;
-  const int t0 = part * per, t1 = min(t0 + per, tiles_all);
+  const int per = part_keys(seen_max, split), parts_used = seen_max > per ? (seen_max + per - 1) / per : 1;
+  if (part >= parts_used) return;
+  const int t0 = part * (per / KT), t1 = min(t0 + per / KT, tiles_all);
   const int full = seen_min / KT;  // tiles that every row sees whole
+  // the same for this wave's rows: tiles that it sees whole, and the first that it does not see at all
+  const int wave_tok0 = (int)tok_first + (rem + min(wave * 32, tile_rows - 1)) / G;
+  const int wave_tok1 = (int)tok_first + (rem + min(wave * 32 + 31, tile_rows - 1)) / G;
+  const int wave_full = CAUSAL ? max(min(shift + wave_tok0 + 1, sq.nk), 0) / KT : sq.nk / KT;
+  const int wave_end = wave * 32 >= tile_rows ? 0 : CAUSAL ? max(min(shift + wave_tok1 + 1, sq.nk) + KT - 1, 0) / KT
+                                                           : tiles_all;
 
   const Scale sc = scale_of(a.scale);
   v8 qf[KS];
@@ -283,50 +312,46 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
     for (int i = 0; i < KS; ++i) qf[i] = load_q<v8>(q + 16 * i, sc);
   }
 
-  // DMA: instruction i of this wave brings rows [(wave IT + i) RPB, + RPB) of a
-  // tile, lane l of it 16 bytes of row l / CPR; offsets within a tile are 32-bit
-  // (row strides are held below 2^24 elements).  Rows past the last key repeat
-  // it.
+  // DMA: instruction i of this wave brings rows 16 wave + i RPB and on of a tile,
+  // lane l of it 16 bytes of row l / CPR.  The swizzle of those rows is the
+  // lane's own XOR a constant, so that an address is a uniform base and a few
+  // bits; offsets within a tile are 32-bit (token strides are below 2^24
+  // elements).  Rows past the last key repeat it.
+  static_assert(IT * RPB == 16, "a wave brings 16 rows");
   const T* kbase = (const T*)a.k + (int64_t)sq.k0 * a.kst + hk * a.ksh;
   const T* vbase = (const T*)a.v + (int64_t)sq.k0 * a.vst + hk * a.vsh;
-  const int dr = wave * IT * RPB + lane / CPR, dc = lane % CPR;
-  const int kst = (int)a.kst, vst = (int)a.vst;
-  auto k_chunk = [&](int i) {
-    const int c = dc ^ k_swizzle<DP>(dr + i * RPB);
-    return (D == DP ? c : min(c, D / 8 - 1)) * 8;
-  };
-  auto v_chunk = [&](int i) {
-    const int c = dc ^ (v_swizzle<DP, true>(dr + i * RPB) << 1);
-    return (D == DP ? c : min(c, D / 8 - 1)) * 8;
-  };
-  int k_off[IT], v_off[IT];
+  const int dr = lane / CPR, dc = lane % CPR;
+  auto issue = [&](const T* base, int64_t stride, int lane_row, int lane_chunk, int tile, T* stage, auto swizzle) {
+    const int key0 = tile * KT + 16 * wave, left = sq.nk - key0;
+    T* dst = stage + wave * IT * 512;
+    if (tile * KT + KT <= sq.nk) {
+      const T* src = base + (int64_t)key0 * stride;
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    k_off[i] = (dr + i * RPB) * kst + k_chunk(i);
-    v_off[i] = (dr + i * RPB) * vst + v_chunk(i);
-  }
-  auto issue = [&](int tile, T* ks, T* vs) {
-    const int key0 = tile * KT;
-    const T* kt = kbase + (int64_t)key0 * a.kst;
-    const T* vt = vbase + (int64_t)key0 * a.vst;
-    T* kd = ks + wave * IT * 512;
-    T* vd = vs + wave * IT * 512;
-    if (key0 + KT <= sq.nk) {
-#pragma unroll
-      for (int i = 0; i < IT; ++i) load_lds16t(kt + k_off[i], kd + i * 512);
-#pragma unroll
-      for (int i = 0; i < IT; ++i) load_lds16t(vt + v_off[i], vd + i * 512);
+      for (int i = 0; i < IT; ++i) {
+        const int c = lane_chunk ^ swizzle(i * RPB);
+        load_lds16t(src + (uint32_t)(lane_row + (D == DP ? c : min(c, D / 8 - 1)) * 8), dst + i * 512);
+        src += RPB * stride;
+      }
     } else {
-      const int end = sq.nk - 1 - key0;
+      const T* src = base + (int64_t)min(key0, sq.nk - 1) * stride;
 #pragma unroll
-      for (int i = 0; i < IT; ++i) load_lds16t(kt + (min(dr + i * RPB, end) * kst + k_chunk(i)), kd + i * 512);
-#pragma unroll
-      for (int i = 0; i < IT; ++i) load_lds16t(vt + (min(dr + i * RPB, end) * vst + v_chunk(i)), vd + i * 512);
+      for (int i = 0; i < IT; ++i) {
+        const int c = lane_chunk ^ swizzle(i * RPB), r = max(min(dr + i * RPB, left - 1), 0);
+        load_lds16t(src + (uint32_t)(r * (int)stride + (D == DP ? c : min(c, D / 8 - 1)) * 8), dst + i * 512);
+      }
     }
+  };
+  const int k_row = dr * (int)a.kst, v_row = dr * (int)a.vst;
+  const int k_chunk = dc ^ k_swizzle<DP>(dr), v_chunk = dc ^ (v_swizzle<DP, true>(dr) << 1);
+  auto issue_k = [&](int tile, T* ks) {
+    issue(kbase, a.kst, k_row, k_chunk, tile, ks, [](int r) { return k_swizzle<DP>(r); });
+  };
+  auto issue_v = [&](int tile, T* vs) {
+    issue(vbase, a.vst, v_row, v_chunk, tile, vs, [](int r) { return v_swizzle<DP, true>(r) << 1; });
   };
 
   float16_t o[DB];
-  float m, l;
+  float m, l;  // reference point of the row's exponentials in log2, sum of its weights
   // lanes' places in the LDS rows
   const int tr_row = 4 * lh + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   auto v_at = [&](const T* vs, int row, int db) {
@@ -341,44 +366,87 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
     for (int i = 0; i < DB; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    if (t0 < t1) issue(t0, k_lds0, v_lds0);
+    if (t0 < t1) {
+      issue_k(t0, k_lds0);
+      issue_v(t0, v_lds0);
+    }
     auto step = [&](int t, const T* ks, T* vs, T* next_k, T* next_v) {
       wait_vmcnt<0>();
       stage_barrier();  // tile t has landed; every wave is done with the other stage
-      if (t + 1 < t1) issue(t + 1, next_k, next_v);
+      if (t + 1 < t1) {
+        issue_k(t + 1, next_k);
+        issue_v(t + 1, next_v);
+      }
       if (careful && t >= full) {
         for (int i = tid; i < STAGE / 8; i += 64 * NW) zero_nonfinite(vs + 8 * i);
         stage_barrier();
       }
+      if (t >= wave_end) return;
+      // K fragments are read four slices at a time and V's a 16-key step ahead, the
+      // first before the softmax: left to itself, the compiler reads each just
+      // before its MFMA and waits.  (Eight slices and two steps ahead spill
+      // registers: 8 texts of 1,024 tokens, 32 / 8 heads of 128: 113 -> 104 us,
+      // 8,192 tokens of 16 / 4 heads of 256: 1,189 -> 702 us.)
       float16_t x[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[kb][e] = 0.f;
-        const int row = kb * 32 + lr;
+      constexpr int KC = KS < 4 ? KS : 4;
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          const v8 kf = *reinterpret_cast<const v8*>(ks + row * DP + (((2 * i + lh) ^ k_swizzle<DP>(row)) << 3));
-          x[kb] = Elem<T>::mfma32(kf, qf[i], x[kb]);
-        }
+      for (int c = 0; c < KS; c += KC) {
+        v8 kf[KC][2];
+#pragma unroll
+        for (int i = 0; i < KC && c + i < KS; ++i)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const int row = kb * 32 + lr;
+            kf[i][kb] = *reinterpret_cast<const v8*>(ks + row * DP + (((2 * (c + i) + lh) ^ k_swizzle<DP>(row)) << 3));
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < KC && c + i < KS; ++i)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) x[kb] = Elem<T>::mfma32(kf[i][kb], qf[c + i], x[kb]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (t >= full) {
-        const int key0 = t * KT + 4 * lh;
+      v8 vf[4][DB];
+      auto read_step = [&](int st) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          vf[st][db] = read_v<T>(v_at(vs, 16 * st + tr_row, db), v_at(vs, 16 * st + 8 + tr_row, db));
+      };
+      read_step(0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t >= wave_full) {
+        const int end = last - t * KT - 4 * lh;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            x[kb][e] = key0 + kb * 32 + 8 * (e >> 2) + (e & 3) > last ? -INFINITY : x[kb][e];
+          for (int e = 0; e < 16; ++e) x[kb][e] = end < kb * 32 + 8 * (e >> 2) + (e & 3) ? -INFINITY : x[kb][e];
       }
       float top = x[0][0];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
-      top = fmaxf(m, pair_max(top));
-      const float base = (top == -INFINITY ? 0.f : top) * sc.c;
-      const float shrink = __builtin_amdgcn_exp2f(m * sc.c - base);
-      m = top;
+      top = pair_max(top) * sc.c;
+      // The reference point of a row's exponentials follows its maximum only where
+      // that has grown by more than 2^8: weights up to 256 are as exact as those
+      // up to 1, and most tiles then leave the sums as they are.  (Each row by its
+      // own scores; rows that do not move are multiplied by 1.)
+      const bool grow = top > m + 8.0f;
+      if (__ballot(grow) != 0) {
+        const float next = grow ? top : m;
+        const float shrink = next == m ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= shrink;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[i][e] *= shrink;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
       v8 p[4];
       float sum = 0.f;
 #pragma unroll
@@ -389,18 +457,15 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
           sum += w;
           p[2 * kb + (e >> 3)][e & 7] = (T)w;
         }
-      l = l * shrink + sum;
+      l += sum;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < DB; ++i)
+      for (int st = 0; st < 4; ++st) {
+        if (st + 1 < 4) read_step(st + 1);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] *= shrink;
-#pragma unroll
-      for (int st = 0; st < 4; ++st)
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const v8 vf = read_v<T>(v_at(vs, 16 * st + tr_row, db), v_at(vs, 16 * st + 8 + tr_row, db));
-          o[db] = Elem<T>::mfma32(vf, p[st], o[db]);
-        }
+        for (int db = 0; db < DB; ++db) o[db] = Elem<T>::mfma32(vf[st][db], p[st], o[db]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     for (int t = t0; t < t1; t += 2) {
       step(t, k_lds0, v_lds0, k_lds1, v_lds1);
@@ -428,18 +493,16 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
   l = pair_sum(l);
   if (!live) return;
   const bool none = last < 0;
-  if (split > 1) {
+  if (parts_used > 1) {
     float* dst = parts + (((int64_t)(sq.q0 + tok) * a.Hq + head) * split + part) * part_stride(D);
-    if (t0 < t1) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4_t*>(dst + db * 32 + 8 * g + 4 * lh) =
-              (float4_t){o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-    }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4_t*>(dst + db * 32 + 8 * g + 4 * lh) =
+            (float4_t){o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
     if (lh == 0) {
-      dst[D] = m * sc.c;
+      dst[D] = m;
       dst[D + 1] = l;
     }
     return;
@@ -462,7 +525,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
 // ---------------------------------------------------------------------------
 template <class T, int D, int RB, int NW>
 __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, int G, int Hk, int k_slots, int chunk,
-                                                        bool only_small, float* parts) {
+                                                        float* parts) {
   typedef typename Elem<T>::v8 v8;
   constexpr int DP = padded(D), KB = 32, R = 16 * RB;
   constexpr int KS = D / 32, DT = D / 16;
@@ -488,13 +551,13 @@ __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, i
     return;
   }
   int64_t first;
-  const int s = sequence_of_slot(a.k_off, (int)a.B, (int)a.Tk, 1, chunk, slot, first);
+  Sequence sq;
+  const int s = sequence_of_slot<true>(a, slot, [&](int o) { return (int64_t)((unsigned)o / (unsigned)chunk); }, first, sq);
   if (s < 0 || s >= a.B) return;
-  const Sequence sq = sequence_at(a, s);
   const int64_t rows = (int64_t)sq.nq * G;
   const int c = (int)(slot - first);
   const bool small = rows <= R;
-  if (rows == 0 || (only_small && !small)) return;
+  if (rows == 0) return;
   // more rows than a tile: the first chunk's workgroup takes all the keys
   if (c > 0 && (!small || (int64_t)c * chunk >= sq.nk)) return;
   const int chunks = small ? max((sq.nk + chunk - 1) / chunk, 1) : 1;
@@ -725,129 +788,162 @@ __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, i
 }
 
 // ---------------------------------------------------------------------------
-// Joins the parts of a row: one wave a query row.
+// Joins the parts of a row: a workgroup a query row, whose groups of L lanes
+// (four columns a lane) take every (256 / L)-th part.
 // ---------------------------------------------------------------------------
-template <class T>
-__global__ __launch_bounds__(256) void join_kernel(PackedAttentionArgs a, int G, int Hk, int small_rows, int chunk,
-                                                   const float* token_parts, int split, const float* prompt_parts) {
-  const int64_t item = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
-  if (item >= a.Tq * a.Hq) return;
-  const int lane = threadIdx.x & 63, D = (int)a.D;
-  const int t = (int)(item / a.Hq), h = (int)(item % a.Hq);
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = 32 * kPromptWaves;
+
+// token_rows: rows of the token kernel's tile (it has written the parts of
+// sequences that fit one), or 0 where the prompt kernel has.
+template <class T, int D>
+__global__ __launch_bounds__(256) void join_kernel(PackedAttentionArgs a, int G, int Hk, int token_rows, int chunk,
+                                                   int split, const float* parts) {
+  constexpr int L = padded(D) / 4, NG = 256 / L, stride = part_stride(D);
+  __shared__ float js[NG][D + 4];
+  const int item = blockIdx.x, Hq = (int)a.Hq;
+  const int t = item / Hq, h = item % Hq;
   const int s = sequence_of_token(a.q_off, (int)a.B, t);
   if (s < 0 || s >= a.B) return;
   const Sequence sq = sequence_at(a, s);
   const int tok = t - sq.q0;
   if (tok < 0 || tok >= sq.nq) return;
-  const int64_t rows = (int64_t)sq.nq * G;
-  const int stride = part_stride(D);
-  const float* src;
+  const int64_t rows = (int64_t)sq.nq * G, r = (int64_t)tok * G + h % G;
   int64_t step;
   int n;
-  if (rows <= small_rows) {
+  if (token_rows > 0) {
     n = (sq.nk + chunk - 1) / chunk;
-    if (n <= 1) return;
-    const int64_t slot = (int64_t)(clamp_to(a.k_off[s], (int)a.Tk) / chunk) + s;
-    step = (int64_t)Hk * small_rows * stride;
-    src = token_parts + ((slot * Hk + h / G) * small_rows + tok * G + h % G) * (int64_t)stride;
+    if (n <= 1 || rows > token_rows) return;
+    const int64_t slot = (int64_t)(sq.k0 / chunk) + s;
+    step = (int64_t)Hk * token_rows * stride;
+    parts += ((slot * Hk + h / G) * token_rows + r) * stride;
   } else {
-    n = split;
-    if (n <= 1) return;
+    // (as the prompt kernel counts them for this row's tile)
+    const int64_t tile_end = min((r / kPromptRows + 1) * kPromptRows, rows) - 1;
+    const int seen = a.causal ? max(min(sq.nk - sq.nq + (int)(tile_end / G) + 1, sq.nk), 0) : sq.nk;
+    const int per = part_keys(seen, split);
+    if (seen <= per) return;
+    n = (seen + per - 1) / per;
     step = stride;
-    src = prompt_parts + item * split * stride;
+    parts += (int64_t)item * split * stride;
   }
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 64) top = fmaxf(top, src[i * step + D]);
-  top = wave_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  const int d = 4 * lane;
-  for (int i = 0; i < n; ++i) {
-    const float* p = src + i * step;
-    const float pm = p[D];
-    if (pm == -INFINITY) continue;  // (a part without a key that this row sees: its sums are not written)
-    const float f = __builtin_amdgcn_exp2f(pm - base);
-    sum += p[D + 1] * f;
-    if (d < D) {
-      const float4_t x = *reinterpret_cast<const float4_t*>(p + d);
+  const int g = threadIdx.x / L, d = threadIdx.x % L * 4;
+  float top = -INFINITY, sum = 0.f;
+  float4_t v = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;  // parts in flight
+  for (int i0 = g; i0 < n; i0 += U * NG) {
+    float m[U], l[U];
+    float4_t x[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += x[e] * f;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NG;
+      const float* p = parts + min(i, n - 1) * step;
+      m[u] = i < n ? p[D] : -INFINITY;
+      l[u] = p[D + 1];
+      x[u] = *reinterpret_cast<const float4_t*>(p + (d < D ? d : 0));
+    }
+    float next = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) next = fmaxf(next, m[u]);
+    const float base = next == -INFINITY ? 0.f : next;
+    const float shrink = __builtin_amdgcn_exp2f(top - base);
+    top = next;
+    sum *= shrink;
+    v *= shrink;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float f = __builtin_amdgcn_exp2f(m[u] - base);  // (0 where a part has no key that this row sees)
+      sum = fmaf(l[u], f, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(x[u][e], f, v[e]);
     }
   }
-  const bool none = sq.nk == 0 || (a.causal && sq.nk - sq.nq + tok < 0);
-  if (d < D) {
-    typename Elem<T>::v4 out;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = (T)(none ? 0.f : v[e] / sum);
-    *reinterpret_cast<typename Elem<T>::v4*>((T*)a.out + t * a.ldo + h * D + d) = out;
+  if (d < D) *reinterpret_cast<float4_t*>(&js[g][d]) = v;
+  if (d == 0) {
+    js[g][D] = top;
+    js[g][D + 1] = sum;
   }
+  __syncthreads();
+  if (threadIdx.x >= D / 4) return;
+  const int c = threadIdx.x * 4;
+  top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NG; ++i) top = fmaxf(top, js[i][D]);
+  const float base = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+  v = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const float f = __builtin_amdgcn_exp2f(js[i][D] - base);
+    const float4_t x = *reinterpret_cast<const float4_t*>(&js[i][c]);
+    sum = fmaf(js[i][D + 1], f, sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+  }
+  const bool none = sq.nk == 0 || (a.causal && sq.nk - sq.nq + tok < 0);
+  typename Elem<T>::v4 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(none ? 0.f : v[e] / sum);
+  *reinterpret_cast<typename Elem<T>::v4*>((T*)a.out + t * a.ldo + h * D + c) = out;
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-constexpr int kPromptWaves = 4;
-constexpr int kPromptRows = 32 * kPromptWaves;
+// (pieces of 257, 1 and 64 tokens against 8,448, 4,099 and 64 keys: 39.4, 40.1, 42.2, 41.8 us
+// with 8, 12, 16, 32 parts; 8 times 4 tokens against 8,192 keys: 44.4, 38.1, 38.6, 38.2)
+constexpr int kMaxSplit = 12;
 constexpr int kTokenExtra = 4;  // workgroups a key head for the rows of no sequence
 
 Plan plan_of(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
   Plan p;
   const int64_t G = Hq / Hk;
   const int64_t cus = device_cu_count();
-  // Rows a sequence: with Tk = Tq the sequences are whole prompts (their keys
-  // are their queries), otherwise those of one token, or of few, meet a cache.
-  const int64_t mean_q = B > 0 ? (Tq + B - 1) / B : 0;
-  const bool cached = Tk > Tq || Tq <= B;
-  if (B > 0 && G <= (D <= 128 ? 64 : 32) && (cached || Tq * G <= 16)) {
-    // room for the group of one token, and of up to four where the batch has them
-    const int64_t few = G * std::min<int64_t>(mean_q, 4);
-    const int64_t r = few <= (D <= 128 ? 64 : 32) ? few : G;
-    p.rb = r <= 16 ? 1 : r <= 32 ? 2 : 4;
-  }
-  // every sequence small, or (but for sequences without queries) of one token
-  const bool all_small = p.rb > 0 && (Tq * G <= 16 * p.rb || Tq <= B);
-  p.prompt = !all_small;
-  if (B == 1 && p.prompt) p.rb = 0;
-  if (p.rb > 0) {
+  // The token kernel where no sequence can have more rows than its tile, or
+  // where there are as many queries as sequences: one each (should one have
+  // more, a workgroup takes all of its keys, tile after tile).
+  const int64_t room = D <= 128 ? 64 : 32;
+  if (B > 0 && (Tq * G <= room || (Tq == B && G <= room))) {
+    const int64_t rows = Tq == B ? G : Tq * G;
+    p.rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     // four workgroups a CU over all keys, at least 512 keys each
     const int64_t want = (Tk * Hk + 4 * cus - 1) / (4 * cus);
     p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 512), 1 << 30);
     p.k_slots = Tk / p.chunk + B + 1;
-    if (Tk > p.chunk) p.token_floats = p.k_slots * Hk * 16 * p.rb * part_stride((int)D);
+    if (Tk > p.chunk) p.floats = p.k_slots * Hk * 16 * p.rb * part_stride((int)D);
+    return p;
   }
-  if (p.prompt) {
-    const int64_t tiles = (Tq * G + kPromptRows - 1) / kPromptRows * Hk;
-    const int64_t mean_k = B > 0 ? Tk / B : 0;
-    // fewer tiles than CUs: the keys of each are split, at least 512 a part
-    if (tiles < cus) p.split = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / tiles, mean_k / 512, 16}));
-    if (p.split > 1) p.prompt_floats = Tq * Hq * p.split * part_stride((int)D);
+  // Fewer tiles than two a CU and long keys: each tile's keys are split.
+  const int64_t tiles = std::max((Tq * G + kPromptRows - 1) / kPromptRows, std::min(B, Tq)) * Hk;
+  if (B > 0 && Tk / B >= 1024 && tiles > 0 && tiles < 2 * cus) {
+    p.split = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / tiles, kMaxSplit));
+    if (p.split > 1) p.floats = Tq * Hq * p.split * part_stride((int)D);
   }
   return p;
 }
 
 template <class T, int D>
-int launch_prompt(const PackedAttentionArgs& a, const Plan& p, int G, int small_rows, float* parts, hipStream_t stream) {
+int launch_prompt(const PackedAttentionArgs& a, const Plan& p, int G, hipStream_t stream) {
   const int64_t slots = a.Tq * G / kPromptRows + a.B + 2;
   const int64_t blocks = slots * a.Hk * p.split;
   if (blocks > 0x7fffffff) return fail(GD_ERR_SHAPE, "packed_attention: too many tiles");
   const dim3 grid((unsigned)blocks), block(64 * kPromptWaves);
+  float* parts = static_cast<float*>(a.workspace);
   if (a.causal)
-    prompt_kernel<T, D, kPromptWaves, true><<<grid, block, 0, stream>>>(a, G, (int)a.Hk, (int)slots, p.split,
-                                                                       small_rows, parts);
+    prompt_kernel<T, D, kPromptWaves, true><<<grid, block, 0, stream>>>(a, G, (int)a.Hk, (int)slots, p.split, parts);
   else
-    prompt_kernel<T, D, kPromptWaves, false><<<grid, block, 0, stream>>>(a, G, (int)a.Hk, (int)slots, p.split,
-                                                                        small_rows, parts);
+    prompt_kernel<T, D, kPromptWaves, false><<<grid, block, 0, stream>>>(a, G, (int)a.Hk, (int)slots, p.split, parts);
   GD_LAUNCH_CHECK();
   return GD_OK;
 }
 
 template <class T, int D, int RB>
-int launch_token(const PackedAttentionArgs& a, const Plan& p, int G, float* parts, hipStream_t stream) {
+int launch_token(const PackedAttentionArgs& a, const Plan& p, int G, hipStream_t stream) {
   constexpr int NW = D <= 128 && RB <= 2 ? 8 : 4;
-  const int64_t blocks = (p.k_slots + (a.zero_rest && !p.prompt ? kTokenExtra : 0)) * a.Hk;
+  const int64_t blocks = (p.k_slots + (a.zero_rest ? kTokenExtra : 0)) * a.Hk;
   if (blocks > 0x7fffffff) return fail(GD_ERR_SHAPE, "packed_attention: too many key chunks");
   token_kernel<T, D, RB, NW><<<dim3((unsigned)blocks), dim3(64 * NW), 0, stream>>>(
-      a, G, (int)a.Hk, (int)p.k_slots, p.chunk, p.prompt, parts);
+      a, G, (int)a.Hk, (int)p.k_slots, p.chunk, static_cast<float*>(a.workspace));
   GD_LAUNCH_CHECK();
   return GD_OK;
 }
@@ -855,18 +951,16 @@ int launch_token(const PackedAttentionArgs& a, const Plan& p, int G, float* part
 template <class T, int D>
 int launch_sized(const PackedAttentionArgs& a, const Plan& p, hipStream_t stream) {
   const int G = (int)(a.Hq / a.Hk);
-  float* token_parts = static_cast<float*>(a.workspace);
-  float* prompt_parts = token_parts + p.token_floats;
-  if (p.rb == 1) GD_RETURN_IF_ERROR((launch_token<T, D, 1>(a, p, G, token_parts, stream)));
-  if (p.rb == 2) GD_RETURN_IF_ERROR((launch_token<T, D, 2>(a, p, G, token_parts, stream)));
+  if (p.rb == 0) GD_RETURN_IF_ERROR((launch_prompt<T, D>(a, p, G, stream)));
+  if (p.rb == 1) GD_RETURN_IF_ERROR((launch_token<T, D, 1>(a, p, G, stream)));
+  if (p.rb == 2) GD_RETURN_IF_ERROR((launch_token<T, D, 2>(a, p, G, stream)));
   if constexpr (D <= 128)
-    if (p.rb == 4) GD_RETURN_IF_ERROR((launch_token<T, D, 4>(a, p, G, token_parts, stream)));
-  if (p.prompt) GD_RETURN_IF_ERROR((launch_prompt<T, D>(a, p, G, 16 * p.rb, prompt_parts, stream)));
-  if (p.token_floats > 0 || p.split > 1) {
-    const int64_t blocks = (a.Tq * a.Hq + 3) / 4;
+    if (p.rb == 4) GD_RETURN_IF_ERROR((launch_token<T, D, 4>(a, p, G, stream)));
+  if (p.floats > 0) {
+    const int64_t blocks = a.Tq * a.Hq;
     if (blocks > 0x7fffffff) return fail(GD_ERR_SHAPE, "packed_attention: too many rows");
-    join_kernel<T><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, G, (int)a.Hk, 16 * p.rb, p.chunk, token_parts,
-                                                                     p.split, prompt_parts);
+    join_kernel<T, D><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, G, (int)a.Hk, 16 * p.rb, p.chunk, p.split,
+                                                                     static_cast<const float*>(a.workspace));
     GD_LAUNCH_CHECK();
   }
   return GD_OK;
@@ -887,21 +981,17 @@ int launch(const PackedAttentionArgs& a, const Plan& p, hipStream_t stream) {
 }  // namespace
 
 int64_t packed_attention_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
-  const Plan p = plan_of(B, Tq, Tk, Hq, Hk, D);
-  return (p.token_floats + p.prompt_floats) * (int64_t)sizeof(float);
+  return plan_of(B, Tq, Tk, Hq, Hk, D).floats * (int64_t)sizeof(float);
 }
 
 int launch_packed_attention(const PackedAttentionArgs& a, hipStream_t stream) {
   Plan p = plan_of(a.B, a.Tq, a.Tk, a.Hq, a.Hk, a.D);
-  if (a.workspace_bytes < (p.token_floats + p.prompt_floats) * (int64_t)sizeof(float)) {
+  if (a.workspace_bytes < p.floats * (int64_t)sizeof(float)) {
     // no room for parts: whole sequences
-    if (p.rb > 0 && p.token_floats > 0) {
-      p.chunk = 1 << 30;
-      p.k_slots = a.Tk / p.chunk + a.B + 1;
-      p.token_floats = 0;
-    }
+    p.chunk = 1 << 30;
+    p.k_slots = a.Tk / p.chunk + a.B + 1;
     p.split = 1;
-    p.prompt_floats = 0;
+    p.floats = 0;
   }
   return a.bf16 ? launch<bf16_t>(a, p, stream) : launch<half_t>(a, p, stream);
 }
