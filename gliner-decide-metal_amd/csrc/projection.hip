@@ -3,15 +3,17 @@
 // Sums are fp32 on the matrix cores (few rows: fp32 multiply-adds), the
 // epilogue works on them in fp32 and rounds once.  Kernels:
 //   * tile_kernel, many rows: a BM x BN tile of 32x32x16 MFMA sub-tiles, 64-wide
-//     K steps brought into LDS by DMA two stages deep (rows of 16-byte
+//     K steps brought into LDS by DMA two to four stages deep (rows of 16-byte
 //     alignment) or through registers (any alignment), the tile staged through
 //     LDS in fp32 so that the epilogue loads the residual and stores the
 //     output in whole 16-byte pieces of rows;
-//   * strip_kernel, up to 64 rows: W is read once, straight from global memory
-//     into the MFMA operands; the waves of a workgroup share a strip of 16 or
-//     32 columns and split K;
+//   * strip_kernel, up to 32 rows: W is read once, straight from global memory
+//     into the MFMA operands; the waves of a workgroup share a strip of 16
+//     columns and split K;
 //   * row_kernel, up to 4 rows: a wave a column or two, lanes along K.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "elem16.hpp"
 #include "gd_kernels.hpp"
@@ -19,19 +21,19 @@
 namespace gd {
 namespace {
 
-// 0.5 erfc(|y| / sqrt(2)) as t q(t) exp(-y^2 / 2), t = 1 / (1 + 0.51 |y| / sqrt(2)),
-// q a minimax fit of erfcx over [0, 10]: 9e-7 of its value everywhere, so GELU's
-// lower tail keeps its digits.
+// 0.5 erfc(|y| / sqrt(2)) as t q(t) exp(-y^2 / 2), t = 1 / (1 + 0.436 |y| / sqrt(2)),
+// q a minimax fit of erfcx over [0, 10]: with the rounding of the exponent within
+// 1e-5 of its value everywhere (a 50th of half a step of fp16), so GELU's lower
+// tail keeps its digits.
 __device__ __forceinline__ float half_erfc(float y) {
   const float z = fabsf(y);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.51f * 0.70710678f, z, 1.0f));
-  float q = 0.04725245f;
-  q = fmaf(q, t, -0.17957604f);
-  q = fmaf(q, t, 0.17923456f);
-  q = fmaf(q, t, 0.02751835f);
-  q = fmaf(q, t, 0.13953599f);
-  q = fmaf(q, t, 0.14207563f);
-  q = fmaf(q, t, 0.14395879f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.436f * 0.70710678f, z, 1.0f));
+  float q = -0.07528479f;
+  q = fmaf(q, t, 0.18845460f);
+  q = fmaf(q, t, 0.00833212f);
+  q = fmaf(q, t, 0.13616963f);
+  q = fmaf(q, t, 0.11909175f);
+  q = fmaf(q, t, 0.12323473f);
   return q * t * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
 }
 
@@ -97,12 +99,15 @@ __device__ __forceinline__ void load_bias(const ProjectionArgs& a, int64_t col, 
 // ---------------------------------------------------------------------------
 constexpr int kBK = 64;
 
+template <int V>
+using ic = std::integral_constant<int, V>;
+
 // LDS rows of 64 elements (128 bytes): 16-byte chunk c of row r at chunk
 // c ^ ((r / 2) & 7), so that the 16 rows of a fragment read at one chunk cover
 // the 64 banks.
 __device__ __forceinline__ int tile_offset(int row, int chunk) { return row * kBK + ((chunk ^ ((row >> 1) & 7)) << 3); }
 
-template <class T, int BM, int BN, int WAVES_M, int NW, int ACT, bool DMA>
+template <class T, int BM, int BN, int WAVES_M, int NW, int NST, int ACT, bool DMA>
 __global__ __launch_bounds__(64 * NW) void tile_kernel(ProjectionArgs a, int tiles_m, int tiles_n) {
   typedef typename Elem<T>::v8 v8;
   constexpr int NT = 64 * NW, WAVES_N = NW / WAVES_M;
@@ -115,6 +120,16 @@ __global__ __launch_bounds__(64 * NW) void tile_kernel(ProjectionArgs a, int til
   // stage being read and leaves the DMA into the other in flight)
   __shared__ __attribute__((aligned(1024))) T st0[STAGE];
   __shared__ __attribute__((aligned(1024))) T st1[STAGE];
+  __shared__ __attribute__((aligned(16))) T st2[NST > 2 ? STAGE : 8];
+  __shared__ __attribute__((aligned(16))) T st3[NST > 3 ? STAGE : 8];
+  static_assert(NST >= 2 && NST <= 4 && NST * STAGE * 2 <= 160 * 1024 && (NST - 1) * LPS < 64, "stages");
+  auto stage = [&](auto i) -> T* {
+    constexpr int I = decltype(i)::value % NST;
+    if constexpr (I == 0) return st0;
+    else if constexpr (I == 1) return st1;
+    else if constexpr (I == 2) return st2;
+    else return st3;
+  };
 
   // Tile order: workgroups go round the 8 XCDs; each XCD takes a run of the
   // tiles in bands of four tile rows, whose x rows and w rows its L2 then serves.
@@ -222,32 +237,42 @@ __global__ __launch_bounds__(64 * NW) void tile_kernel(ProjectionArgs a, int til
     };
     // Every step issues one stage (past the last step that one again, which
     // nobody reads), so each wait is for a constant number of loads.
-    auto step = [&](T* st, const T* next, int t) {
+    auto step = [&](auto i, int t) {
+      constexpr int I = decltype(i)::value;
+      T* const st = stage(i);
 #pragma unroll
       for (int s = 0; s < 3; ++s) {
         read_frags(st, s + 1, (s + 1) & 1);
         mma(s & 1);
         interleave();
       }
-      wait_vmcnt<0>();
+      wait_vmcnt<(NST - 2) * LPS>();
       stage_barrier();  // the next stage has landed, this one is in everyone's registers
-      issue(st, t + 2);
-      read_frags(next, 0, 0);
+      issue(st, t + NST);
+      read_frags(stage(ic<I + 1>{}), 0, 0);
       mma(1);
       interleave();
     };
     if (steps > 0) {
       issue(st0, 0);
       issue(st1, 1);
-      wait_vmcnt<LPS>();
+      if constexpr (NST > 2) issue(st2, 2);
+      if constexpr (NST > 3) issue(st3, 3);
+      wait_vmcnt<(NST - 1) * LPS>();
       stage_barrier();
       read_frags(st0, 0, 0);
+      // (whole rounds of the stages without a branch, which would cost a wait for
+      // every load in flight)
       int t = 0;
-      for (; t + 2 <= steps; t += 2) {
-        step(st0, st1, t);
-        step(st1, st0, t + 1);
+      for (; t + NST <= steps; t += NST) {
+        step(ic<0>{}, t);
+        step(ic<1>{}, t + 1);
+        if constexpr (NST > 2) step(ic<2>{}, t + 2);
+        if constexpr (NST > 3) step(ic<3>{}, t + 3);
       }
-      if (t < steps) step(st0, st1, t);
+      if (t < steps) step(ic<0>{}, t);
+      if constexpr (NST > 2) if (t + 1 < steps) step(ic<1>{}, t + 1);
+      if constexpr (NST > 3) if (t + 2 < steps) step(ic<2>{}, t + 2);
       wait_vmcnt<0>();
       __syncthreads();
     }
@@ -311,7 +336,7 @@ __global__ __launch_bounds__(64 * NW) void tile_kernel(ProjectionArgs a, int til
 
 // ---------------------------------------------------------------------------
 // Few rows: 16 RB rows of x against a strip of 16 columns (rows of w); the NW
-// waves take every NW-th 32-wide step of K.  Operands come from global memory
+// waves take every NW-th block of 128 columns of K.  Operands come from global memory
 // as they are (x from the L2).  Rows past the last repeat it.
 // ---------------------------------------------------------------------------
 template <class T, int RB, int NW, int ACT>
@@ -320,23 +345,23 @@ __global__ __launch_bounds__(64 * NW) void strip_kernel(ProjectionArgs a) {
   __shared__ float part[NW][16 * RB][17];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 15, lg = lane >> 4;
-  const int64_t n0 = blockIdx.x * (int64_t)16, m0 = blockIdx.y * (int64_t)(16 * RB);
+  const int64_t n0 = blockIdx.x * (int64_t)16;
   const T* w = (const T*)a.w + min(n0 + lc, a.n - 1) * a.ldw;
   const T* x[RB];
   float4_t acc[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    x[b] = (const T*)a.x + min(m0 + 16 * b + lc, a.m - 1) * a.ldx;
+    x[b] = (const T*)a.x + min((int64_t)(16 * b + lc), a.m - 1) * a.ldx;
     acc[b] = (float4_t){0.f, 0.f, 0.f, 0.f};
   }
-  const int64_t steps = a.k / 32;
-  constexpr int U = 4;  // steps in flight
-  int64_t t = wave;
-  for (; t + (U - 1) * NW < steps; t += U * NW) {
+  // blocks of U steps (whole 128-byte lines of a row) in flight, every NW-th a wave's
+  constexpr int U = 4;
+  int64_t k0 = wave * (32 * U);
+  for (; k0 + 32 * U <= a.k; k0 += NW * 32 * U) {
     v8 fw[U], fx[U][RB];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int64_t k = (t + i * NW) * 32 + 8 * lg;
+      const int64_t k = k0 + i * 32 + 8 * lg;
       fw[i] = load8(w + k);
 #pragma unroll
       for (int b = 0; b < RB; ++b) fx[i][b] = load8(x[b] + k);
@@ -346,8 +371,8 @@ __global__ __launch_bounds__(64 * NW) void strip_kernel(ProjectionArgs a) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) acc[b] = Elem<T>::mfma16(fw[i], fx[i][b], acc[b]);
   }
-  for (; t * 32 < a.k; t += NW) {
-    const int64_t k = t * 32 + 8 * lg;
+  for (const int64_t end = min(k0 + 32 * U, a.k); k0 < end; k0 += 32) {  // the wave that has the last, short block
+    const int64_t k = k0 + 8 * lg;
     const int left = (int)max(min(a.k - k, (int64_t)8), (int64_t)0);
     const v8 fw = load8(w + k, left);
 #pragma unroll
@@ -361,13 +386,13 @@ __global__ __launch_bounds__(64 * NW) void strip_kernel(ProjectionArgs a) {
   __syncthreads();
   for (int i = tid; i < 16 * RB * 16; i += 64 * NW) {
     const int r = i >> 4, c = i & 15;
-    if (m0 + r >= a.m || n0 + c >= a.n) continue;
+    if (r >= a.m || n0 + c >= a.n) continue;
     float v = 0.f;
 #pragma unroll
     for (int j = 0; j < NW; ++j) v += part[j][r][c];
     float bias;
     load_bias<T, 1>(a, n0 + c, &bias);
-    finish<T, ACT, 1>(a, m0 + r, n0 + c, &v, &bias);
+    finish<T, ACT, 1>(a, r, n0 + c, &v, &bias);
   }
 }
 
@@ -431,14 +456,53 @@ __global__ __launch_bounds__(256) void row_kernel(ProjectionArgs a) {
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-template <class T, int BM, int BN, int WAVES_M, int NW, int ACT, bool DMA>
+template <class T, int BM, int BN, int WAVES_M, int NW, int NST, int ACT, bool DMA>
 int launch_tile(const ProjectionArgs& a, hipStream_t stream) {
   const int64_t tm = (a.m + BM - 1) / BM, tn = (a.n + BN - 1) / BN;
   if (tm * tn > 0x7fffffff || tn > 0x1fffffff) return fail(GD_ERR_SHAPE, "projection: too many tiles");
-  tile_kernel<T, BM, BN, WAVES_M, NW, ACT, DMA>
+  tile_kernel<T, BM, BN, WAVES_M, NW, NST, ACT, DMA>
       <<<dim3((unsigned)(tm * tn)), dim3(64 * NW), 0, stream>>>(a, (int)tm, (int)tn);
   GD_LAUNCH_CHECK();
   return GD_OK;
+}
+
+// Tiles by the time that they would take, in us: a round of one workgroup a CU
+// takes e + s a K step, where two fit, a round of two e2 + s2, and one that is
+// partly of two a part of the way between.  The numbers are fits to 14 shapes
+// of 128 to 8,192 rows, 1,024 to 4,096 columns and K of 1,024 and 4,096 on 256
+// CUs (bf16 onto a residual), within 25% of the times measured and mostly 10%:
+// 8,192 x 4,096 x 4,096 takes 238, 292, 355, 436 us with the four tiles, 2,048 x
+// 4,096 x 1,024 35, 26, 30, 36, 2,048 x 1,024 x 4,096 83, 42, 25, 28, 512 x
+// 1,024 x 4,096 83, 42, 23, 16.
+int tile_choice(int64_t m, int64_t n, int64_t k) {
+  struct Tile {
+    int bm, bn;
+    double e, s, e2, s2;  // e2 = 0: one workgroup a CU
+  };
+  static const Tile kTiles[4] = {{256, 256, 13.5, 1.1, 0, 0.6},  // (s grows by s2 as the CUs fill up)
+                                 {128, 128, 3.5, 0.62, 8.5, 0.98},
+                                 {128, 64, 4.0, 0.32, 5.0, 0.61},
+                                 {64, 64, 3.5, 0.20, 4.5, 0.37}};
+  const double cus = device_cu_count(), steps = (double)((k + kBK - 1) / kBK);
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 4; ++i) {
+    const Tile& t = kTiles[i];
+    const double tiles = (double)((m + t.bm - 1) / t.bm) * (double)((n + t.bn - 1) / t.bn);
+    const double slots = t.e2 > 0 ? 2 * cus : cus, full = std::floor(tiles / slots), rest = tiles - full * slots;
+    double time;
+    if (t.e2 > 0) {
+      const double one = t.e + t.s * steps, two = t.e2 + t.s2 * steps;
+      time = full * two;
+      if (rest > cus) time += one + (two - one) * (0.4 + 0.6 * (rest - cus) / cus);
+      else if (rest > 0) time += one;
+    } else {
+      time = full * (t.e + (t.s + t.s2) * steps);
+      if (rest > 0) time += t.e + (t.s + t.s2 * rest / cus) * steps;
+    }
+    if (i == 0 || time < least) best = i, least = time;
+  }
+  return best;
 }
 
 template <class T, int ACT>
@@ -454,15 +518,17 @@ int launch_act(const ProjectionArgs& a, hipStream_t stream) {
     GD_LAUNCH_CHECK();
     return GD_OK;
   }
-  if (a.m <= 64) {
-    const int64_t strips = (a.n + 15) / 16;
-    const dim3 grid((unsigned)strips, 1);
+  // Strips up to 32 rows and two workgroups a CU, where 64 x 64 tiles leave most
+  // CUs idle: 16 x 4,096 x 4,096 10.6 against 15.1 us, 32 rows 13.1 against 15.2, 16
+  // x 4,096 x 16,384 38 against 57; 48 rows 18.0 against 15.7, 16 x 16,384 x 4,096
+  // 31.6 against 22.8.
+  const int64_t strips = (a.n + 15) / 16;
+  if (a.m <= 32 && strips <= 2 * device_cu_count()) {
+    const dim3 grid((unsigned)strips);
     if (a.m <= 16)
       strip_kernel<T, 1, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
-    else if (a.m <= 32)
-      strip_kernel<T, 2, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
     else
-      strip_kernel<T, 4, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
+      strip_kernel<T, 2, 8, ACT><<<grid, dim3(512), 0, stream>>>(a);
     GD_LAUNCH_CHECK();
     return GD_OK;
   }
@@ -470,12 +536,13 @@ int launch_act(const ProjectionArgs& a, hipStream_t stream) {
   auto rows16 = [](const void* p, int64_t ld) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 23);
   };
-  if (!rows16(a.x, a.ldx) || !rows16(a.w, a.ldw)) return launch_tile<T, 128, 128, 2, 4, ACT, false>(a, stream);
-  const int64_t cus = device_cu_count();
-  auto tiles = [&](int bm, int bn) { return (a.m + bm - 1) / bm * ((a.n + bn - 1) / bn); };
-  if (tiles(256, 256) >= cus) return launch_tile<T, 256, 256, 2, 8, ACT, true>(a, stream);
-  if (tiles(128, 128) >= cus) return launch_tile<T, 128, 128, 2, 4, ACT, true>(a, stream);
-  return launch_tile<T, 64, 64, 2, 4, ACT, true>(a, stream);
+  if (!rows16(a.x, a.ldx) || !rows16(a.w, a.ldw)) return launch_tile<T, 128, 128, 2, 4, 2, ACT, false>(a, stream);
+  switch (tile_choice(a.m, a.n, a.k)) {
+    case 0: return launch_tile<T, 256, 256, 2, 8, 2, ACT, true>(a, stream);
+    case 1: return launch_tile<T, 128, 128, 2, 4, 2, ACT, true>(a, stream);
+    case 2: return launch_tile<T, 128, 64, 2, 4, 3, ACT, true>(a, stream);
+    default: return launch_tile<T, 64, 64, 2, 4, 4, ACT, true>(a, stream);
+  }
 }
 
 template <class T>
