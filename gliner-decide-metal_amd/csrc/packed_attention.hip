@@ -382,41 +382,53 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
         stage_barrier();
       }
       if (t >= wave_end) return;
-      // K fragments are read four slices at a time and V's a 16-key step ahead, the
-      // first before the softmax: left to itself, the compiler reads each just
-      // before its MFMA and waits.  (Eight slices and two steps ahead spill
-      // registers: 8 texts of 1,024 tokens, 32 / 8 heads of 128: 113 -> 104 us,
-      // 8,192 tokens of 16 / 4 heads of 256: 1,189 -> 702 us.)
+      // K fragments are read three slices ahead of their MFMAs and V's four MFMAs
+      // ahead, the first of them before the softmax, in the order that the group
+      // barriers give: left to itself, the compiler reads each just before its MFMA
+      // and waits.  (16,384 tokens of 32 / 8 heads of 128 2,115 -> 2,052 us against
+      // batches of eight reads, 8,192 of 16 / 4 heads of 256 692 -> 657 us.)
       float16_t x[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[kb][e] = 0.f;
-      constexpr int KC = KS < 4 ? KS : 4;
-#pragma unroll
-      for (int c = 0; c < KS; c += KC) {
-        v8 kf[KC][2];
-#pragma unroll
-        for (int i = 0; i < KC && c + i < KS; ++i)
+      {
+        v8 kf[KS][2];
+        auto read_k = [&](int i) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb) {
             const int row = kb * 32 + lr;
-            kf[i][kb] = *reinterpret_cast<const v8*>(ks + row * DP + (((2 * (c + i) + lh) ^ k_swizzle<DP>(row)) << 3));
+            kf[i][kb] = *reinterpret_cast<const v8*>(ks + row * DP + (((2 * i + lh) ^ k_swizzle<DP>(row)) << 3));
           }
+        };
+        constexpr int AH = KS < 3 ? KS : 3;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < KC && c + i < KS; ++i)
+        for (int i = 0; i < AH; ++i) read_k(i);
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) x[kb] = Elem<T>::mfma32(kf[i][kb], qf[c + i], x[kb]);
+        for (int i = 0; i < KS; ++i) {
+          if (i + AH < KS) read_k(i + AH);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) x[kb] = Elem<T>::mfma32(kf[i][kb], qf[i], x[kb]);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * AH, 0);
+#pragma unroll
+        for (int i = 0; i < KS - AH; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * AH, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
-      v8 vf[4][DB];
-      auto read_step = [&](int st) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-          vf[st][db] = read_v<T>(v_at(vs, 16 * st + tr_row, db), v_at(vs, 16 * st + 8 + tr_row, db));
+      v8 vf[4 * DB];
+      auto read_v_at = [&](int i) {
+        const int row = 16 * (i / DB) + tr_row;
+        vf[i] = read_v<T>(v_at(vs, row, i % DB), v_at(vs, row + 8, i % DB));
       };
-      read_step(0);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) read_v_at(i);
       __builtin_amdgcn_sched_barrier(0);
       if (t >= wave_full) {
         const int end = last - t * KT - 4 * lh;
@@ -460,12 +472,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
       l += sum;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        if (st + 1 < 4) read_step(st + 1);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = Elem<T>::mfma32(vf[st][db], p[st], o[db]);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < 4 * DB; ++i) {
+        if (i + DB < 4 * DB) read_v_at(i + DB);
+        o[i % DB] = Elem<T>::mfma32(vf[i], p[i / DB], o[i % DB]);
       }
+#pragma unroll
+      for (int i = 0; i < 3 * DB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, DB, 0);
+      __builtin_amdgcn_sched_barrier(0);
     };
     for (int t = t0; t < t1; t += 2) {
       step(t, k_lds0, v_lds0, k_lds1, v_lds1);
