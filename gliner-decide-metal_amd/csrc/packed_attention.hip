@@ -55,48 +55,70 @@ __device__ __forceinline__ Sequence sequence_at(const PackedAttentionArgs& a, in
   return sequence_of_offsets(a, a.q_off[s], a.q_off[s + 1], a.k_off[s], a.k_off[s + 1]);
 }
 
+// The last entry i of n whose key, key_of(i), is at or before `at`, or -1: each
+// round the lanes look at 64 entries that are a 64th of the rest apart, so up to
+// 64 entries take one trip to memory and 4,096 two.  (Keys do not decrease; if
+// they do, some entry is found.)  After the last round lane l holds what
+// key_of(lo + l) has read; `lo` and `count` say of which entries.
+template <class Key>
+__device__ __forceinline__ int last_at_or_before(int n, int64_t at, Key key_of, int& lo, int& count) {
+  const int lane = threadIdx.x & 63;
+  lo = 0;
+  for (;;) {
+    const int step = (n + 63) / 64;
+    const bool in = lane * (int64_t)step < n;
+    const int64_t key = in ? key_of(lo + lane * step) : INT64_MAX;
+    const int c = __popcll(__ballot(in && key <= at));
+    if (step == 1) {
+      count = n;
+      return lo + c - 1;
+    }
+    if (c == 0) {
+      count = 0;
+      return lo - 1;
+    }
+    lo += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
+  }
+}
+
 // Sequence of a slot: the last i in [0, B] whose first slot, units(offset i) + i,
 // is at or before it; -1 before the first, B behind the last sequence (sq is
 // set for the others).  `first` is the found sequence's first slot (0 for -1).
-// Its offsets come from the lanes that looked: one trip to memory.
+// Its offsets come from the lanes that looked.
 template <bool BY_KEYS, class Units>
 __device__ __forceinline__ int sequence_of_slot(const PackedAttentionArgs& a, int64_t slot, Units units, int64_t& first,
                                                 Sequence& sq) {
-  const int lane = threadIdx.x & 63, B = (int)a.B;
-  for (int i0 = 0;; i0 += 64) {
-    const int i = i0 + lane;
-    const int qo = i <= B ? a.q_off[i] : 0, ko = i <= B ? a.k_off[i] : 0;
-    const int64_t start = i <= B ? units(clamp_to(BY_KEYS ? ko : qo, (int)(BY_KEYS ? a.Tk : a.Tq))) + i : INT64_MAX;
-    const int c = __popcll(__ballot(start <= slot));
-    if (c == 64 && i0 + 64 <= B) continue;
-    const int s = i0 + c - 1;
-    if (s < 0) {
-      first = 0;
-      return -1;
-    }
-    if (c > 0 && c < 64) {
-      const int q0 = __builtin_amdgcn_readlane(qo, c - 1), q1 = __builtin_amdgcn_readlane(qo, c);
-      const int k0 = __builtin_amdgcn_readlane(ko, c - 1), k1 = __builtin_amdgcn_readlane(ko, c);
-      first = units(clamp_to(BY_KEYS ? k0 : q0, (int)(BY_KEYS ? a.Tk : a.Tq))) + s;
-      if (s < B) sq = sequence_of_offsets(a, q0, q1, k0, k1);
-    } else {  // (this and the next offset lie in two rounds)
-      first = units(clamp_to(BY_KEYS ? a.k_off[s] : a.q_off[s], (int)(BY_KEYS ? a.Tk : a.Tq))) + s;
-      if (s < B) sq = sequence_at(a, s);
-    }
-    return s;
+  const int B = (int)a.B;
+  int qo = 0, ko = 0, lo, count;
+  auto first_of = [&](int i, int q, int k) { return units(clamp_to(BY_KEYS ? k : q, (int)(BY_KEYS ? a.Tk : a.Tq))) + i; };
+  const int s = last_at_or_before(
+      B + 1, slot,
+      [&](int i) {
+        qo = a.q_off[i];
+        ko = a.k_off[i];
+        return first_of(i, qo, ko);
+      },
+      lo, count);
+  first = 0;
+  if (s < 0) return -1;
+  const int at = s - lo;  // the lane that has seen it
+  if (at >= 0 && at + 1 < count) {
+    const int q0 = __builtin_amdgcn_readlane(qo, at), q1 = __builtin_amdgcn_readlane(qo, at + 1);
+    const int k0 = __builtin_amdgcn_readlane(ko, at), k1 = __builtin_amdgcn_readlane(ko, at + 1);
+    first = first_of(s, q0, k0);
+    sq = sequence_of_offsets(a, q0, q1, k0, k1);
+  } else {  // (the next offset was not looked at, or there is none)
+    first = first_of(s, a.q_off[s], a.k_off[s]);
+    if (s < B) sq = sequence_at(a, s);
   }
+  return s;
 }
 
 // Sequence of a token: the last i with off[i] <= t, in [-1, B].
 __device__ __forceinline__ int sequence_of_token(const int32_t* off, int B, int t) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int i0 = 0; i0 <= B; i0 += 64) {
-    const int c = __popcll(__ballot(i0 + lane <= B && off[i0 + lane] <= t));
-    n += c;
-    if (c < 64) break;
-  }
-  return n - 1;
+  int lo, count;
+  return last_at_or_before(B + 1, t, [&](int i) { return (int64_t)off[i]; }, lo, count);
 }
 
 // What the host chooses for a call from its numbers alone.
@@ -968,15 +990,14 @@ int launch_token(const PackedAttentionArgs& a, const Plan& p, int G, hipStream_t
 template <class T, int D>
 int launch_sized(const PackedAttentionArgs& a, const Plan& p, hipStream_t stream) {
   const int G = (int)(a.Hq / a.Hk);
+  if (p.floats > 0 && a.Tq * a.Hq > 0x7fffffff) return fail(GD_ERR_SHAPE, "packed_attention: too many rows to join");
   if (p.rb == 0) GD_RETURN_IF_ERROR((launch_prompt<T, D>(a, p, G, stream)));
   if (p.rb == 1) GD_RETURN_IF_ERROR((launch_token<T, D, 1>(a, p, G, stream)));
   if (p.rb == 2) GD_RETURN_IF_ERROR((launch_token<T, D, 2>(a, p, G, stream)));
   if constexpr (D <= 128)
     if (p.rb == 4) GD_RETURN_IF_ERROR((launch_token<T, D, 4>(a, p, G, stream)));
   if (p.floats > 0) {
-    const int64_t blocks = a.Tq * a.Hq;
-    if (blocks > 0x7fffffff) return fail(GD_ERR_SHAPE, "packed_attention: too many rows");
-    join_kernel<T, D><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a, G, (int)a.Hk, 16 * p.rb, p.chunk, p.split,
+    join_kernel<T, D><<<dim3((unsigned)(a.Tq * a.Hq)), dim3(256), 0, stream>>>(a, G, (int)a.Hk, 16 * p.rb, p.chunk, p.split,
                                                                      static_cast<const float*>(a.workspace));
     GD_LAUNCH_CHECK();
   }

@@ -289,7 +289,7 @@ class FusedKernels:
         same_kind(v, q, "v")
         Tq, H, D = q.shape
         Tk, Hk, _ = k.shape
-        if k.shape != v.shape or k.shape[2] != D:
+        if k.shape != v.shape or k.shape[2] != D or D == 0:
             raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"k and v must both be [tokens, kv_heads, {D}]")
         q_offsets, batch = self._offsets(q_offsets, q, "q_offsets")
         if k_offsets is not None:

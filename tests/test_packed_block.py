@@ -312,6 +312,44 @@ def test_attention_long_keys():
 
 
 @gpu
+@pytest.mark.parametrize("batch", [63, 64, 65, 127, 300, 4095, 4096, 4097, 9000])
+def test_attention_many_sequences(batch):
+    """Short sequences by the hundreds and thousands, some empty: prompts, single tokens, tokens with long keys."""
+    r = np.random.default_rng(batch)
+    ql = [int(n) for n in r.integers(0, 4, batch)]
+    q, k, v = normal(1, sum(ql), 2, 32), normal(2, sum(ql), 1, 32), normal(3, sum(ql), 1, 32)
+    seqs = np.repeat(np.arange(batch), ql)
+    starts = np.concatenate([[0], np.cumsum(ql)])
+
+    def check(got, seq_of, k_starts, k_len, pos):
+        """Every row against its own sequence's keys, padded to the longest."""
+        top = int(k_len.max())
+        cols = torch.arange(top, device="cuda")
+        first = torch.from_numpy(k_starts[seq_of]).cuda()
+        idx = (first[:, None] + cols).clamp(max=k2.shape[0] - 1)
+        kk, vv = k2[idx, 0].double(), v2[idx, 0].double()  # [rows, top, D]
+        seen = torch.from_numpy(pos).cuda()[:, None] >= cols
+        for h in range(q2.shape[1]):
+            qq = q2[:, h].double()
+            s = (kk * qq[:, None]).sum(-1) * 32 ** -0.5
+            p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+            want = (p[..., None] * vv).sum(1)
+            av = (p[..., None] * vv.abs()).sum(1)
+            d = 40 * E * ((kk * qq[:, None]).abs().sum(-1) * 32 ** -0.5).amax(-1, keepdim=True)
+            tol = (2.0 ** -11 * want.abs() + TINY[q.dtype] + av * (2.0 ** -11 + 2 * d + 2.0 ** -20 + top * E)
+                   + 2.0 ** -25 * (vv.abs() * seen[..., None]).sum(1))
+            within(got[:, h], want, tol, f"{batch} sequences")
+
+    q2, k2, v2 = q, k, v
+    check(fk().packed_attention(q, k, v, offsets(ql)), seqs, starts, np.asarray(ql),
+          np.arange(len(seqs)) - starts[seqs])
+    kl = r.integers(1, 9, batch)
+    q2, k2, v2 = normal(4, batch, 2, 32), normal(5, int(kl.sum()), 1, 32), normal(6, int(kl.sum()), 1, 32)
+    check(fk().packed_attention(q2, k2, v2, offsets([1] * batch), offsets(kl)), np.arange(batch),
+          np.concatenate([[0], np.cumsum(kl)]), kl, kl - 1)
+
+
+@gpu
 @pytest.mark.parametrize("q_cap,lengths", [(64, ([40, 24], [10, 30, 24])), (2, ([1, 1], [1, 1]))])
 def test_attention_in_a_graph(q_cap, lengths):
     """Captured once, replayed with other offsets and inputs, two graphs in turn, against eager calls."""
