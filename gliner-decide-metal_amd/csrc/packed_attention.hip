@@ -14,20 +14,28 @@
 // from LDS (ds_read_b64_tr_b16) in that same order.
 //   * prompt_kernel, many rows a sequence: tiles of 128 rows (four waves of 32)
 //     on 32x32x16 MFMA, 64 keys a step, K and V straight from global memory
-//     into two LDS stages;
+//     into two LDS stages.  Two workgroups a CU at head width 128.  16,384 tokens
+//     of 32 / 8 heads of 128 (bf16) take 2.05 ms, 1.07 PFLOP/s of the pairs that
+//     the mask leaves: the matrix cores are busy 52% of the cycles, the vector
+//     unit about as long (the exponentials), and the card holds its clock at 1.8
+//     to 2.0 GHz: a form with the scores one tile ahead of the softmax took 7%
+//     fewer cycles at a clock 7% lower.  At head width 64 the exponentials bound it (0.79 PFLOP/s over
+//     8,192 tokens of 16 heads);
 //   * token_kernel, few rows a sequence (16 RB for RB = 1, 2, 4): each wave
 //     walks 32 keys a step on 16x16x32 MFMA, K from global memory into
 //     registers, V into the wave's own LDS; a sequence is cut into chunks of
-//     keys and chunks are joined by join_kernel.
-// The weights are rounded to the tensors' type for P V (half a step of a weight
-// that is at most 1: the output moves by no more than its own rounding does);
-// scores, maxima, sums and the output stay fp32 until the one rounding at the
-// end.
+//     keys and chunks are joined by join_kernel.  HBM bounds it: 16 tokens of 32 /
+//     8 heads of 128 against 145,000 keys read 598 MB in 128 us (4.7 TB/s; a large
+//     copy reaches 5.1), and the join takes 5 us more.
+// The weights are rounded to the tensors' type for P V: the output moves by at
+// most half a step of the type relative to the weighted mean of |v|, as its own
+// rounding does.  Scores, maxima, sums and the output stay fp32 until the one
+// rounding at the end.
 //
 // Workgroups find their sequence from the offsets alone (no plan, no lengths
 // on the host): with s tiles of BM rows before offset o being floor(o / BM),
 // sequence i starts at slot floor(o_i / BM) + i, and has a slot for each of its
-// tiles whatever the lengths are; one ballot over 64 starts finds it.
+// tiles whatever the lengths are.
 #include <algorithm>
 
 #include "elem16.hpp"
@@ -173,7 +181,7 @@ __device__ __forceinline__ void load_lds16t(const T* g, T* lds_block) {
 // not.  Where a row tile had hidden keys and a sum is not finite, the tile is
 // computed again with the infinities and NaN of V set to 0 in the steps with
 // hidden keys (zero_nonfinite, in LDS), and those of the keys that a row sees
-// are added to its sums afterwards (add_nonfinite, from global memory).
+// are added to its sums afterwards (nonfinite_of, from global memory).
 template <class T>
 __device__ __forceinline__ bool nonfinite_bits(unsigned x) {
   constexpr unsigned kExp = __is_same(T, half_t) ? 0x7C00u : 0x7F80u;
@@ -190,7 +198,7 @@ __device__ __forceinline__ void zero_nonfinite(T* v) {
   }
   *reinterpret_cast<uint4_t*>(v) = u;
 }
-// What four values of a seen key add to their sums if they are not finite.
+// What a value of a seen key adds to its sum if it is not finite.
 template <class T>
 __device__ __forceinline__ float nonfinite_of(T v) {
   return nonfinite_bits<T>(__builtin_bit_cast(unsigned short, v)) ? (float)v : 0.f;
@@ -251,8 +259,8 @@ __device__ __forceinline__ int part_keys(int seen, int split) {
 // Many rows a sequence.
 // ---------------------------------------------------------------------------
 template <class T, int D, int NW, bool CAUSAL>
-__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(PackedAttentionArgs a, int G, int Hk, int slots, int split,
-                                                            float* parts) {
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(PackedAttentionArgs a, int G, int Hk,
+                                                                            int slots, int split, float* parts) {
   typedef typename Elem<T>::v8 v8;
   typedef typename Elem<T>::v4 v4;
   constexpr int BM = 32 * NW, KT = 64, DP = padded(D);

@@ -6,11 +6,18 @@
 //     K steps brought into LDS by DMA two to four stages deep (rows of 16-byte
 //     alignment) or through registers (any alignment), the tile staged through
 //     LDS in fp32 so that the epilogue loads the residual and stores the
-//     output in whole 16-byte pieces of rows;
-//   * strip_kernel, up to 32 rows: W is read once, straight from global memory
+//     output in whole 16-byte pieces of rows.  8,192 x 4,096 x 16,384 bf16 onto a
+//     residual: 854 us, 1.29 PFLOP/s, bound by the matrix cores and the card's
+//     power (the vendor library's product alone: 789 us).  8,192 x 4,096 x 1,024
+//     with GELU: 88 us, of which two epilogues of some 14 us run beside no MFMA
+//     (59 us the product alone).  777 x 1,000 x 4,096: 16.5 us, 64 x 64 tiles bound
+//     by what the L2 gives (16.8 TB/s);
+//   * strip_kernel, up to 32 rows (16 x 4,096 x 4,096: 10.6 us): W is read once, straight from global memory
 //     into the MFMA operands; the waves of a workgroup share a strip of 16
 //     columns and split K;
-//   * row_kernel, up to 4 rows: a wave a column or two, lanes along K.
+//   * row_kernel, up to 4 rows: a wave a column, lanes along K; bound by the bytes
+//     of w (1 x 16,384 x 4,096: 20 us, 134 MB, part of them from the last-level
+//     cache).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -397,60 +404,54 @@ __global__ __launch_bounds__(64 * NW) void strip_kernel(ProjectionArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Up to four rows: a wave C columns, 64 lanes x 8 elements of K a step.
+// Up to four rows: a wave a column, 64 lanes x 8 elements of K a step.
 // ---------------------------------------------------------------------------
-template <class T, int M, int C, int ACT>
+template <class T, int M, int ACT>
 __global__ __launch_bounds__(256) void row_kernel(ProjectionArgs a) {
   typedef typename Elem<T>::v8 v8;
   const int lane = threadIdx.x & 63;
-  const int64_t n0 = (blockIdx.x * (int64_t)4 + (threadIdx.x >> 6)) * C;
-  if (n0 >= a.n) return;
-  const T* x = (const T*)a.x;
-  const T* w[C];
+  const int64_t col = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
+  if (col >= a.n) return;
+  const T* w = (const T*)a.w + col * a.ldw;
+  const T* x[M];
 #pragma unroll
-  for (int c = 0; c < C; ++c) w[c] = (const T*)a.w + min(n0 + c, a.n - 1) * a.ldw;
-  float acc[M][C] = {};
-  auto add = [&](const v8* fw, const v8* fx) {
+  for (int m = 0; m < M; ++m) x[m] = (const T*)a.x + min((int64_t)m, a.m - 1) * a.ldx;
+  float acc[M] = {};
+  auto add = [&](v8 fw, const v8* fx) {
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[m][c] = fmaf((float)fw[c][e], (float)fx[m][e], acc[m][c]);
+      for (int e = 0; e < 8; ++e) acc[m] = fmaf((float)fw[e], (float)fx[m][e], acc[m]);
   };
   int64_t k = lane * 8;
   for (; k + 512 + 8 <= a.k; k += 1024) {
-    v8 fw[2][C], fx[2][M];
+    v8 fw[2], fx[2][M];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+      fw[i] = load8(w + k + 512 * i);
 #pragma unroll
-      for (int c = 0; c < C; ++c) fw[i][c] = load8(w[c] + k + 512 * i);
-#pragma unroll
-      for (int m = 0; m < M; ++m) fx[i][m] = load8(x + min((int64_t)m, a.m - 1) * a.ldx + k + 512 * i);
+      for (int m = 0; m < M; ++m) fx[i][m] = load8(x[m] + k + 512 * i);
     }
     add(fw[0], fx[0]);
     add(fw[1], fx[1]);
   }
   for (; k < a.k; k += 512) {
     const int left = (int)min(a.k - k, (int64_t)8);
-    v8 fw[C], fx[M];
+    v8 fx[M];
+    const v8 fw = load8(w + k, left);
 #pragma unroll
-    for (int c = 0; c < C; ++c) fw[c] = load8(w[c] + k, left);
-#pragma unroll
-    for (int m = 0; m < M; ++m) fx[m] = load8(x + min((int64_t)m, a.m - 1) * a.ldx + k, left);
+    for (int m = 0; m < M; ++m) fx[m] = load8(x[m] + k, left);
     add(fw, fx);
   }
 #pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float v = wave_sum_dpp(acc[m][c]);
-      if (lane == m * C + c && m < a.m && n0 + c < a.n) {
-        float bias;
-        load_bias<T, 1>(a, n0 + c, &bias);
-        finish<T, ACT, 1>(a, m, n0 + c, &v, &bias);
-      }
+  for (int m = 0; m < M; ++m) {
+    float v = wave_sum_dpp(acc[m]);
+    if (lane == m && m < a.m) {
+      float bias;
+      load_bias<T, 1>(a, col, &bias);
+      finish<T, ACT, 1>(a, m, col, &v, &bias);
     }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -510,11 +511,11 @@ int launch_act(const ProjectionArgs& a, hipStream_t stream) {
   if (a.m <= 4) {
     const int64_t blocks = (a.n + 3) / 4;
     if (a.m == 1)
-      row_kernel<T, 1, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
+      row_kernel<T, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
     else if (a.m == 2)
-      row_kernel<T, 2, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
+      row_kernel<T, 2, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
     else
-      row_kernel<T, 4, 1, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
+      row_kernel<T, 4, ACT><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(a);
     GD_LAUNCH_CHECK();
     return GD_OK;
   }

@@ -185,6 +185,23 @@ def test_attention_rising_and_falling_scores(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("heads,kv_heads,dim,ql,kl", [
+    (16, 2, 64, [3, 0, 0], [2000, 5, 700]),  # as many queries as sequences, but one sequence has them all
+    (32, 4, 128, [0, 5, 0, 0, 0], [10, 3000, 1, 1, 900]),
+    (80, 1, 64, [1, 1], [300, 2000]),  # a group of more heads than the token tile's rows
+    (40, 1, 256, [1, 1, 1], [1500, 7, 64]),
+    (64, 1, 128, [1, 1], [1030, 2500]),
+    (24, 3, 96, [2], [1400]),
+    (12, 2, 128, [257, 1, 64], [2448, 1099, 64]),
+])
+def test_attention_uneven_batches(heads, kv_heads, dim, ql, kl):
+    for causal in (True, False):
+        q = normal(1, sum(ql), heads, dim)
+        k, v = normal(2, sum(kl), kv_heads, dim), normal(3, sum(kl), kv_heads, dim)
+        check_attention(q, k, v, ql, kl, causal)
+
+
+@gpu
 def test_attention_views():
     """Parts of one projection's output, heads before tokens, int64 offsets, rows wider than the heads."""
     ql = [37, 1, 140]
