@@ -537,7 +537,13 @@ int launch_act(const ProjectionArgs& a, hipStream_t stream) {
   auto rows16 = [](const void* p, int64_t ld) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 23);
   };
-  if (!rows16(a.x, a.ldx) || !rows16(a.w, a.ldw)) return launch_tile<T, 128, 128, 2, 4, 2, ACT, false>(a, stream);
+  if (!rows16(a.x, a.ldx) || !rows16(a.w, a.ldw)) {
+    // (128 and 64 wide: 300 x 1,000 x 1,001 27 and 12 us, 3,784 x 502 x 3,126 103 and 40,
+    // 148 x 192 x 3,711 79 and 35)
+    const int64_t tiles = (a.m + 127) / 128 * ((a.n + 127) / 128);
+    return tiles < device_cu_count() ? launch_tile<T, 64, 64, 2, 4, 2, ACT, false>(a, stream)
+                                     : launch_tile<T, 128, 128, 2, 4, 2, ACT, false>(a, stream);
+  }
   switch (tile_choice(a.m, a.n, a.k)) {
     case 0: return launch_tile<T, 256, 256, 2, 8, 2, ACT, true>(a, stream);
     case 1: return launch_tile<T, 128, 128, 2, 4, 2, ACT, true>(a, stream);
