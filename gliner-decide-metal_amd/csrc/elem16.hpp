@@ -1,5 +1,5 @@
 // The two 16-bit element types of the packed-row operators: vector types,
-// conversions to and from fp32 (round to nearest even) and the MFMA forms.
+// the MFMA forms, and a sum of two elements onto fp32 (subnormal elements count).
 #pragma once
 
 #include "gd_common.hpp"
@@ -22,6 +22,9 @@ struct Elem<half_t> {
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float add2(v2 a, float c) {
+    return __builtin_amdgcn_fdot2(a, (v2){(half_t)1.f, (half_t)1.f}, c, false);
+  }
 };
 
 template <>
@@ -34,6 +37,9 @@ struct Elem<bf16_t> {
   }
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(v2 a, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(a, (v2){(bf16_t)1.f, (bf16_t)1.f}, c, false);
   }
 };
 

@@ -27,10 +27,11 @@
 //     keys and chunks are joined by join_kernel.  HBM bounds it: 16 tokens of 32 /
 //     8 heads of 128 against 145,000 keys read 598 MB in 128 us (4.7 TB/s; a large
 //     copy reaches 5.1), and the join takes 5 us more.
-// The weights are rounded to the tensors' type for P V: the output moves by at
-// most half a step of the type relative to the weighted mean of |v|, as its own
-// rounding does.  Scores, maxima, sums and the output stay fp32 until the one
-// rounding at the end.
+// The weights are rounded to the tensors' type for P V and, so rounded, summed (in
+// fp32): the output stays a mean of the values with weights that are off by at
+// most half a step of the type, a constant value comes out as itself, and the
+// sum takes half the instructions.  Scores, maxima, sums and the output stay fp32
+// until the one rounding at the end.
 //
 // Workgroups find their sequence from the offsets alone (no plan, no lengths
 // on the host): with s tiles of BM rows before offset o being floor(o / BM),
@@ -263,6 +264,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
                                                                             int slots, int split, float* parts) {
   typedef typename Elem<T>::v8 v8;
   typedef typename Elem<T>::v4 v4;
+  typedef typename Elem<T>::v2 v2;
   constexpr int BM = 32 * NW, KT = 64, DP = padded(D);
   constexpr int KS = D / 16, DB = D / 32;       // K slices of a score, 32-wide blocks of d
   constexpr int CPR = DP / 8;                   // 16-byte chunks of an LDS row
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
       // ahead, the first of them before the softmax, in the order that the group
       // barriers give: left to itself, the compiler reads each just before its MFMA
       // and waits.  (16,384 tokens of 32 / 8 heads of 128 2,115 -> 2,052 us against
-      // batches of eight reads, 8,192 of 16 / 4 heads of 256 692 -> 657 us.)
+      // batches of eight reads, 8,192 of 16 / 4 heads of 256 692 -> 638 us.)
       float16_t x[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -457,8 +459,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
         const int row = 16 * (i / DB) + tr_row;
         vf[i] = read_v<T>(v_at(vs, row, i % DB), v_at(vs, row + 8, i % DB));
       };
+      constexpr int VA = DB < 4 ? DB : 4;
 #pragma unroll
-      for (int i = 0; i < DB; ++i) read_v_at(i);
+      for (int i = 0; i < VA; ++i) read_v_at(i);
       __builtin_amdgcn_sched_barrier(0);
       if (t >= wave_full) {
         const int end = last - t * KT - 4 * lh;
@@ -490,28 +493,28 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void prompt_kernel(Packe
       }
       const float base = m == -INFINITY ? 0.f : m;
       v8 p[4];
-      float sum = 0.f;
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float w = __builtin_amdgcn_exp2f(x[kb][e] * sc.c - base);
-          sum += w;
-          p[2 * kb + (e >> 3)][e & 7] = (T)w;
-        }
-      l += sum;
+      for (int i = 0; i < 32; i += 2) {
+        const v2 w = {(T)__builtin_amdgcn_exp2f(x[i >> 4][i & 15] * sc.c - base),
+                      (T)__builtin_amdgcn_exp2f(x[i >> 4][(i & 15) + 1] * sc.c - base)};
+        sum[(i >> 1) & 1] = Elem<T>::add2(w, sum[(i >> 1) & 1]);
+        p[i >> 3][i & 7] = w[0];
+        p[i >> 3][(i & 7) + 1] = w[1];
+      }
+      l += sum[0] + sum[1];
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 4 * DB; ++i) {
-        if (i + DB < 4 * DB) read_v_at(i + DB);
+        if (i + VA < 4 * DB) read_v_at(i + VA);
         o[i % DB] = Elem<T>::mfma32(vf[i], p[i / DB], o[i % DB]);
       }
 #pragma unroll
-      for (int i = 0; i < 3 * DB; ++i) {
+      for (int i = 0; i < 4 * DB - VA; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, DB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, VA, 0);
       __builtin_amdgcn_sched_barrier(0);
     };
     for (int t = t0; t < t1; t += 2) {
@@ -718,10 +721,12 @@ __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, i
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float w = __builtin_amdgcn_exp2f(x[b][kb][e] * sc.c - base);
-              sum += w;
-              p[b][4 * kb + e] = (T)w;
+            for (int e = 0; e < 4; e += 2) {
+              const typename Elem<T>::v2 w = {(T)__builtin_amdgcn_exp2f(x[b][kb][e] * sc.c - base),
+                                              (T)__builtin_amdgcn_exp2f(x[b][kb][e + 1] * sc.c - base)};
+              sum = Elem<T>::add2(w, sum);
+              p[b][4 * kb + e] = w[0];
+              p[b][4 * kb + e + 1] = w[1];
             }
           l[b] = l[b] * shrink + sum;
 #pragma unroll

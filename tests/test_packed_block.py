@@ -4,10 +4,12 @@ block run through all of them.
 
 Tolerances.  u is half a step of the output's type relative to its value
 (fp16 2^-11, bf16 2^-8, fp32 2^-24), e = 2^-24 that of the fp32 arithmetic.
-  attention   The weights p are rounded to the type for P.V, so the sum moves
-              by at most u * sum p|v| (fp16 also by 2^-25 a key below its
-              normal range, with the largest p at least 1), the output by
-              u |out| (and 2^-25).  A score of D products moves by
+  attention   The weights p are rounded to the type, for P.V and for their
+              sum: with p (1 + r), |r| <= u, the output moves by sum r p (v -
+              out) / sum p, at most u (sum p|v| / sum p + |out|) (fp16 also by
+              2^-25 (|v| + |out|) a key below its normal range, with the
+              largest p at least 1), and by u |out| (and 2^-25) when it is
+              rounded itself.  A score of D products moves by
               d = (D + 8) e scale sum|q k|, a weight by twice that of the
               worst key and 2^-20 for the exponential, the sums by n e.
   projection  (k + 8) e sum|x w| before the activation, whose slope is at most
@@ -89,10 +91,10 @@ def attention_reference(q, k, v, q_lengths, k_lengths, scale, causal):
             o = (p @ vv) / total
             av = (p @ vv.abs()) / total
             d = (D + 8) * E * mag.amax(-1, keepdim=True)
-            t = u * o.abs() + TINY[q.dtype] + av * (u + 2 * d + 2.0 ** -20 + nk * E)
+            t = 2 * u * o.abs() + TINY[q.dtype] + av * (u + 2 * d + 2.0 ** -20 + nk * E)
             if q.dtype == torch.float16:
                 visible = (~torch.isinf(s)).double()
-                t = t + 2.0 ** -25 * (visible @ vv.abs())
+                t = t + 2.0 ** -25 * (visible @ vv.abs() + visible.sum(-1, keepdim=True) * o.abs())
             out[q0:q0 + nq, h] = torch.where(some, o, 0.0)
             tol[q0:q0 + nq, h] = torch.where(some, t, 0.0)
         q0 += nq
@@ -281,6 +283,32 @@ def test_attention_hidden_values_have_no_effect(dtype, bad):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,value", [(torch.float16, 65504.0), (torch.float16, -65504.0), (torch.float16, 6e-8),
+                                         (torch.bfloat16, 1e30), (torch.bfloat16, 0.3)])
+def test_attention_of_constant_values(dtype, value):
+    """Equal values come out as they are, the type's largest among them, and none where nothing is seen."""
+    for ql, kl in (([200, 30], [200, 30]), ([1, 1], [700, 3]), ([5, 130], [2000, 1500]), ([9], [4])):
+        q, k = normal(1, sum(ql), 6, 64, dtype=dtype), normal(2, sum(kl), 2, 64, dtype=dtype)
+        v = torch.full_like(k, value)
+        got = fk().packed_attention(q, k, v, offsets(ql), offsets(kl))
+        want = torch.full_like(got, value)
+        if ql == [9]:
+            want[:5] = 0.0
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@gpu
+def test_attention_of_no_queries_or_keys():
+    q, k, v = normal(1, 6, 4, 64), normal(2, 9, 2, 64), normal(3, 9, 2, 64)
+    kernels = fk()
+    assert not kernels.packed_attention(q, k[:0], v[:0], offsets([2, 4]), offsets([0, 0])).any()
+    assert not kernels.packed_attention(q[:2], k[:0], v[:0], offsets([1, 1]), offsets([0, 0])).any()
+    assert kernels.packed_attention(q[:0], k, v, offsets([0]), offsets([9])).shape == (0, 4, 64)
+    assert kernels.packed_attention(q[:0], k[:0], v[:0], offsets([])).shape == (0, 4, 64)
+
+
+@gpu
 def test_attention_rows_do_not_depend_on_their_neighbours():
     """A sequence's rows have the same bits alone and in a batch of its kind, twice over."""
     ql = [65, 200, 129]
@@ -353,8 +381,8 @@ def test_attention_many_sequences(batch):
             want = (p[..., None] * vv).sum(1)
             av = (p[..., None] * vv.abs()).sum(1)
             d = 40 * E * ((kk * qq[:, None]).abs().sum(-1) * 32 ** -0.5).amax(-1, keepdim=True)
-            tol = (2.0 ** -11 * want.abs() + TINY[q.dtype] + av * (2.0 ** -11 + 2 * d + 2.0 ** -20 + top * E)
-                   + 2.0 ** -25 * (vv.abs() * seen[..., None]).sum(1))
+            tol = (2.0 ** -10 * want.abs() + TINY[q.dtype] + av * (2.0 ** -11 + 2 * d + 2.0 ** -20 + top * E)
+                   + 2.0 ** -25 * ((vv.abs() * seen[..., None]).sum(1) + seen.sum(-1, keepdim=True) * want.abs()))
             within(got[:, h], want, tol, f"{batch} sequences")
 
     q2, k2, v2 = q, k, v
