@@ -87,7 +87,7 @@ def call_on(t: torch.Tensor, fn, *args) -> None:
     """fn(*args, current stream) on t's device, whichever device is current."""
     index = t.get_device()
     if index == _current_device():
-        status = fn(*args, stream_handle())
+        status = fn(*args, stream_handle() if _raw_stream is None else _raw_stream(index))
     else:
         with torch.cuda.device(index):
             status = fn(*args, stream_handle())

@@ -55,10 +55,14 @@ _ACTIVATIONS = {"none": N.GD_ACT_NONE, "relu": N.GD_ACT_RELU, "gelu": N.GD_ACT_G
 _NORMS = {"layer": N.GD_NORM_LAYER, "rms": N.GD_NORM_RMS}
 
 
+_NO_ROWS = N.GdRows(None, 0)
+
+
 def _choice(table: dict, key, name: str) -> int:
-    if key not in table:
+    code = table.get(key)
+    if code is None:
         raise N.GlinerDecideError(N.GD_ERR_INVALID_ARGUMENT, f"{name} must be one of {', '.join(table)} (got {key!r})")
-    return table[key]
+    return code
 
 
 def _tokens(t: torch.Tensor, name: str) -> N.GdTokens:
@@ -285,11 +289,13 @@ class FusedKernels:
         only: the result carries no gradient."""
         dtype = dtype16(q, "q")
         qt, kt, vt = _tokens(q, "q"), _tokens(k, "k"), _tokens(v, "v")
-        same_kind(k, q, "k")
-        same_kind(v, q, "v")
+        qd, dev = q.dtype, q.get_device()
+        if k.dtype is not qd or v.dtype is not qd or k.get_device() != dev or v.get_device() != dev:
+            same_kind(k, q, "k")
+            same_kind(v, q, "v")
         Tq, H, D = q.shape
-        Tk, Hk, _ = k.shape
-        if k.shape != v.shape or k.shape[2] != D or D == 0:
+        Tk, Hk, Dk = k.shape
+        if k.shape != v.shape or Dk != D or D == 0:
             raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"k and v must both be [tokens, kv_heads, {D}]")
         q_offsets, batch = self._offsets(q_offsets, q, "q_offsets")
         if k_offsets is not None:
@@ -298,7 +304,7 @@ class FusedKernels:
                 raise N.GlinerDecideError(N.GD_ERR_SHAPE, "q_offsets and k_offsets must have one length")
         flags = N.GD_PACKED_CAUSAL if causal else 0
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty((Tq, H, D), dtype=qd, device=q.device)
             ldo = H * D
             flags |= N.GD_PACKED_ZERO_REST
         else:
@@ -318,9 +324,9 @@ class FusedKernels:
             raise ValueError(f"{name} must be on {like.device} (got {t.device})")
         if t.dtype is not torch.int32 or not t.is_contiguous():
             t = as_i32(t, name)
-        if t.dim() != 1 or t.shape[0] < 1:
+        if t.dim() != 1 or t.numel() < 1:
             raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"{name} must be [batch + 1] (got {tuple(t.shape)})")
-        return t, t.shape[0] - 1
+        return t, t.numel() - 1
 
     def projection(self, x, weight, bias=None, residual=None, *, activation: str = "none", scale: float = 1.0,
                    out: torch.Tensor | None = None) -> torch.Tensor:
@@ -333,19 +339,19 @@ class FusedKernels:
         dtype = dtype16(x, "x")
         same_kind(weight, x, "weight")
         n, K = _dims(weight, 2, "weight")
-        if x.dim() < 1 or x.shape[-1] != K:
-            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"x {tuple(x.shape)} does not end in the weight's {K} columns")
+        xs = x.shape
+        if not xs or xs[-1] != K:
+            raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"x {tuple(xs)} does not end in the weight's {K} columns")
         act = _choice(_ACTIVATIONS, activation, "activation")
-        shape = x.shape[:-1] + (n,)
+        shape = (xs[0], n) if len(xs) == 2 else (*xs[:-1], n)
         x2, xr = _rows(x, K)
         w2, wr = _rows(weight, K)
         bias = _vector(bias, x, (n,), "bias")
-        res = N.GdRows(None, 0)
+        res = _NO_ROWS
         if residual is not None:
             same_kind(residual, x, "residual")
             if residual.shape != shape:
-                raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"residual must be {tuple(shape)} (got "
-                                                          f"{tuple(residual.shape)})")
+                raise N.GlinerDecideError(N.GD_ERR_SHAPE, f"residual must be {shape} (got {tuple(residual.shape)})")
             residual, res = _rows(residual, n)
         if out is None:
             out, ldo = torch.empty(shape, dtype=x.dtype, device=x.device), n
@@ -378,18 +384,23 @@ class FusedKernels:
         if pre_weight is None:
             raise N.GlinerDecideError(N.GD_ERR_INVALID_ARGUMENT, "pre_weight is needed")
         vec = (C,)
-        pre_w, pre_b = _vector(pre_weight, y, vec, "pre_weight"), _vector(pre_bias, y, vec, "pre_bias")
-        post_w, post_b = _vector(post_weight, y, vec, "post_weight"), _vector(post_bias, y, vec, "post_bias")
+        pre_w = _vector(pre_weight, y, vec, "pre_weight")
+        pre_b = None if pre_bias is None else _vector(pre_bias, y, vec, "pre_bias")
+        post_w = None if post_weight is None else _vector(post_weight, y, vec, "post_weight")
+        post_b = None if post_bias is None else _vector(post_bias, y, vec, "post_bias")
         y2, yr = _rows(y, C)
         r2, rr = _rows(residual, C)
-        g, per_gate = N.GdRows(None, 0), 1
+        g, per_gate = _NO_ROWS, 1
         if gate is not None:
             same_kind(gate, y, "gate")
             gate, per_gate = self._gate_rows(gate, shape, rows)
             gate, g = _rows(gate, C)
         if out is None:
-            h = torch.empty_like(residual, memory_format=torch.contiguous_format)
-            n = torch.empty_like(y, memory_format=torch.contiguous_format)
+            # (r2 and y2 are rows: contiguous ones need no format named)
+            h = torch.empty_like(r2) if r2 is residual and r2.is_contiguous() else torch.empty(
+                shape, dtype=residual.dtype, device=y.device)
+            n = torch.empty_like(y2) if y2 is y and y2.is_contiguous() else torch.empty(
+                shape, dtype=y.dtype, device=y.device)
             ldh = ldn = C
         else:
             h, n = out
