@@ -7,10 +7,10 @@
 //     alignment) or through registers (any alignment), the tile staged through
 //     LDS in fp32 so that the epilogue loads the residual and stores the
 //     output in whole 16-byte pieces of rows.  8,192 x 4,096 x 16,384 bf16 onto a
-//     residual: 854 us, 1.29 PFLOP/s, bound by the matrix cores and the card's
+//     residual: 854 to 875 us, 1.26 to 1.29 PFLOP/s, bound by the matrix cores and the card's
 //     power (the vendor library's product alone: 789 us).  8,192 x 4,096 x 1,024
-//     with GELU: 88 us, of which two epilogues of some 14 us run beside no MFMA
-//     (59 us the product alone).  777 x 1,000 x 4,096: 16.5 us, 64 x 64 tiles bound
+//     with GELU: 87 us, of which two epilogues of some 14 us run beside no MFMA
+//     (74 us without an activation, the library's product alone 59).  777 x 1,000 x 4,096: 16.5 us, 64 x 64 tiles bound
 //     by what the L2 gives (16.8 TB/s);
 //   * strip_kernel, up to 32 rows (16 x 4,096 x 4,096: 10.6 us): W is read once, straight from global memory
 //     into the MFMA operands; the waves of a workgroup share a strip of 16
@@ -72,20 +72,27 @@ __device__ __forceinline__ typename Elem<T>::v8 load8(const T* p, int n = 8) {
 }
 
 // Epilogue of N consecutive elements of a row from column col (those below n).
-template <class T, int ACT, int N>
+template <class T, int ACT, int N, bool STREAM = false>
 __device__ __forceinline__ void finish(const ProjectionArgs& a, int64_t row, int64_t col, const float* acc,
                                        const float* bias) {
   const T* res = a.residual ? (const T*)a.residual + row * a.ldr + col : nullptr;
   T* out = (T*)a.out + row * a.ldo + col;
-  T r[N];
-  if (col + N <= a.n) {
-    if (res) __builtin_memcpy(r, res, 2 * N);
+  if (N == 8 && col + N <= a.n) {
+    // One load and one store of 16 bytes at any alignment; STREAM: past the operand
+    // tiles in the L2 (8,192 x 4,096 x 1,024: 81.9 -> 75.0 us without an activation, 92.0
+    // -> 90.1 with GELU, against stores of 12 and 2 bytes; 75.7 and 91.6 not streamed).
+    typedef T piece __attribute__((ext_vector_type(8), aligned(2)));
+    piece r, add = {};
+    if (res) add = *reinterpret_cast<const piece*>(res);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float y = a.scale * activate<ACT>(acc[e] + bias[e]);
-      r[e] = (T)(res ? y + (float)r[e] : y);
+      r[e] = (T)(res ? y + (float)add[e] : y);
     }
-    __builtin_memcpy(out, r, 2 * N);
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(r, reinterpret_cast<piece*>(out));
+    else
+      *reinterpret_cast<piece*>(out) = r;
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -335,7 +342,7 @@ __global__ __launch_bounds__(64 * NW) void tile_kernel(ProjectionArgs a, int til
       float v[8];
       *reinterpret_cast<float4_t*>(v) = *reinterpret_cast<const float4_t*>(src + 4 * ((2 * u) ^ (r & 15)));
       *reinterpret_cast<float4_t*>(v + 4) = *reinterpret_cast<const float4_t*>(src + 4 * ((2 * u + 1) ^ (r & 15)));
-      finish<T, ACT, 8>(a, m0 + first + r, n0 + 8 * u, v, bias);
+      finish<T, ACT, 8, BM == 256>(a, m0 + first + r, n0 + 8 * u, v, bias);
     }
     __syncthreads();
   }

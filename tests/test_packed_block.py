@@ -884,7 +884,7 @@ def test_block_norm_in_a_graph_and_far_rows():
     for i, t in enumerate(far):
         t.copy_(normal(20 + i, rows, 1024))
     other = torch.empty((rows, stride), dtype=torch.float16, device="cuda")
-    check_block_norm(far[0], far[1], (w, None), (w, None), far[2], out=(other[:, :1024], other[:, 2048:3072]))
+    check_block_norm(far[0], far[1], (w, None), (w, None), far[2], out=(other[:, :1024], other[:, 4096:5120]))
 
 
 def _norm_status(y=(FAKE, 64), res=(2 * FAKE, 64), gate=(None, 0), per=1, post_w=3 * FAKE, post_b=None, pre_w=4 * FAKE,
