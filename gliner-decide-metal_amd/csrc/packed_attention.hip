@@ -250,6 +250,12 @@ __device__ __forceinline__ void zero_rows(const PackedAttentionArgs& a, int hk, 
   }
 }
 
+// First place for the parts of a sequence of more than one chunk whose keys start
+// at k0: 2 floor(k0 / chunk).  It has ceil(n / chunk) parts, at most floor(n /
+// chunk) + 1 <= 2 floor(n / chunk), so the next such sequence starts behind them,
+// and 2 floor(tokens / chunk) + 2 places hold all, however many sequences there are.
+__device__ __forceinline__ int64_t part_slot(int k0, int chunk) { return 2 * (int64_t)(k0 / chunk); }
+
 // Keys of a part where a tile of the prompt kernel sees `seen` keys and has
 // room for `split` parts: whole steps, at least four.
 __device__ __forceinline__ int part_keys(int seen, int split) {
@@ -820,7 +826,7 @@ __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, i
         const int64_t row = rb0 + r;
         const int tok = (int)(row / G), head = hk * G + (int)(row % G);
         if (chunks > 1) {
-          float* part = parts + ((slot * Hk + hk) * R + 16 * b + r) * part_stride(D);
+          float* part = parts + (((part_slot(sq.k0, chunk) + c) * Hk + hk) * R + 16 * b + r) * part_stride(D);
           *reinterpret_cast<float4_t*>(part + d) = v;
           if (d == 0) {
             part[D] = top;
@@ -866,9 +872,8 @@ __global__ __launch_bounds__(256) void join_kernel(PackedAttentionArgs a, int G,
   if (token_rows > 0) {
     n = (sq.nk + chunk - 1) / chunk;
     if (n <= 1 || rows > token_rows) return;
-    const int64_t slot = (int64_t)(sq.k0 / chunk) + s;
     step = (int64_t)Hk * token_rows * stride;
-    parts += ((slot * Hk + h / G) * token_rows + r) * stride;
+    parts += ((part_slot(sq.k0, chunk) * Hk + h / G) * token_rows + r) * stride;
   } else {
     // (as the prompt kernel counts them for this row's tile)
     const int64_t tile_end = min((r / kPromptRows + 1) * kPromptRows, rows) - 1;
@@ -962,7 +967,7 @@ Plan plan_of(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t 
     const int64_t want = (Tk * Hk + 4 * cus - 1) / (4 * cus);
     p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 512), 1 << 30);
     p.k_slots = Tk / p.chunk + B + 1;
-    if (Tk > p.chunk) p.floats = p.k_slots * Hk * 16 * p.rb * part_stride((int)D);
+    if (Tk > p.chunk) p.floats = (2 * (Tk / p.chunk) + 2) * Hk * 16 * p.rb * part_stride((int)D);
     return p;
   }
   // Fewer tiles than two a CU and long keys: each tile's keys are split.

@@ -348,8 +348,9 @@ def test_attention_far_offsets(nq):
 
 @gpu
 def test_attention_long_keys():
-    """One token against 70,000 keys, and three sequences of very unequal length."""
-    for kl in ([70000], [9, 40000, 700]):
+    """One token against 70,000 keys, sequences of very unequal length, chunks that end everywhere."""
+    for kl in ([70000], [9, 40000, 700], [513, 511, 1024, 1025, 1, 0, 1537, 512, 2047, 3], [600] * 40,
+               [2000 + 37 * i for i in range(24)]):
         ql = [1] * len(kl)
         q = normal(1, len(kl), 8, 128, dtype=torch.bfloat16)
         k, v = (normal(s, sum(kl), 1, 128, dtype=torch.bfloat16) for s in (2, 3))
@@ -497,6 +498,13 @@ def _attention_status(q=(FAKE, 512, 64), k=(2 * FAKE, 128, 64), v=(3 * FAKE, 128
 def test_attention_refusals(status, kwargs):
     assert _attention_status(**kwargs) == status
     assert N.last_error()
+
+
+@pytest.mark.parametrize("batch", [1, 16, 4096, 1 << 20])
+def test_attention_workspace_does_not_grow_with_the_batch(batch):
+    """Single tokens over 2^28 keys in all: parts for the chunks, not for every sequence."""
+    size = N.lib().gd_packed_attention_workspace(batch, batch, 1 << 28, 32, 8, 128)
+    assert 0 < size <= 64 << 20
 
 
 def test_attention_of_nothing_without_device():
