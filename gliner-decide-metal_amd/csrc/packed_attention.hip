@@ -614,10 +614,13 @@ __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, i
   const int c = (int)(slot - first);
   const bool small = rows <= R;
   if (rows == 0) return;
-  // more rows than a tile: the first chunk's workgroup takes all the keys
-  if (c > 0 && (!small || (int64_t)c * chunk >= sq.nk)) return;
-  const int chunks = small ? max((sq.nk + chunk - 1) / chunk, 1) : 1;
-  const int key_lo = c * chunk, key_hi = chunks > 1 ? min(key_lo + chunk, sq.nk) : sq.nk;
+  // More rows than a tile (a batch of as many queries as sequences, one of which
+  // has several): the chunks' workgroups share the row tiles, each over all keys.
+  const int slots_used = max((sq.nk + chunk - 1) / chunk, 1);
+  if (c >= slots_used) return;
+  const int chunks = small ? slots_used : 1;
+  const int key_lo = small ? c * chunk : 0, key_hi = chunks > 1 ? min(key_lo + chunk, sq.nk) : sq.nk;
+  const int64_t row_step = small ? R : (int64_t)slots_used * R;
 
   const int lc = lane & 15, lg = lane >> 4;
   const Scale sc = scale_of(a.scale);
@@ -633,7 +636,7 @@ __global__ __launch_bounds__(64 * NW) void token_kernel(PackedAttentionArgs a, i
     return vs + row * DP + ((dt ^ v_swizzle<DP, false>(row)) << 4) + tr_col;
   };
 
-  for (int64_t row0 = 0; row0 < rows; row0 += R) {
+  for (int64_t row0 = small ? 0 : (int64_t)c * R; row0 < rows; row0 += row_step) {
     int last[RB];
     int last_min = INT_MAX, last_max = -1;
     v8 qf[RB][KS];
@@ -958,7 +961,7 @@ Plan plan_of(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t 
   const int64_t cus = device_cu_count();
   // The token kernel where no sequence can have more rows than its tile, or
   // where there are as many queries as sequences: one each (should one have
-  // more, a workgroup takes all of its keys, tile after tile).
+  // more, its tiles take all of its keys).
   const int64_t room = D <= 128 ? 64 : 32;
   if (B > 0 && (Tq * G <= room || (Tq == B && G <= room))) {
     const int64_t rows = Tq == B ? G : Tq * G;

@@ -190,6 +190,7 @@ def test_attention_rising_and_falling_scores(dtype):
 @pytest.mark.parametrize("heads,kv_heads,dim,ql,kl", [
     (16, 2, 64, [3, 0, 0], [2000, 5, 700]),  # as many queries as sequences, but one sequence has them all
     (32, 4, 128, [0, 5, 0, 0, 0], [10, 3000, 1, 1, 900]),
+    (16, 2, 64, [0, 40] + [0] * 38, [900, 2600] + [7] * 38),
     (80, 1, 64, [1, 1], [300, 2000]),  # a group of more heads than the token tile's rows
     (40, 1, 256, [1, 1, 1], [1500, 7, 64]),
     (64, 1, 128, [1, 1], [1030, 2500]),
